@@ -324,6 +324,64 @@ int ternaspmm_attn_prefill(ternaspmm_bf16* qkv, ternaspmm_bf16* k_cache, ternasp
                            int batch, int tokens, int heads, int kv_heads, int head_dim, int max_len,
                            ternaspmm_stream_t stream);
 
+/* ---- rotary positions, a key / value cache in 4 bits, scores of given tokens -----------------------------
+ * All return the status that ternaspmm_last_status() reports for what the host checks (0, 1 shape, 2 pointer or alignment, 3
+ * launch).  What only the device can see - a position outside of a table or a cache, a token outside of the
+ * vocabulary - is refused by the kernel: status 1 in ternaspmm_last_status(), NaN in the results concerned, caches as they were.
+ * `strides`: elements between two sequences, tokens and heads of a tensor [batch][tokens][heads][head_dim] with contiguous heads. */
+
+/* Queries (and keys, k_heads > 0) rotated by the angles of their positions: pairs (2i, 2i+1) of the first rotary_dim values of a
+ * head, or (i, i + rotary_dim / 2) with half_layout; (a, b) -> (a c - b s, a s + b c), the rest is copied.  inverse: -s (the
+ * gradient).  type: 0 bf16, 1 fp16, 2 fp32.  cos_tab, sin_tab fp32 [table_len][rotary_dim / 2]; pos int64, `pos_batch_stride` and
+ * `pos_token_stride` elements apart (0: shared).  q_out, k_out contiguous.  Any strides in the half layout; even ones, and pointers to whole pairs, in
+ * the other.  head_dim and rotary_dim even. */
+int ternaspmm_rotate(const void* q, const long long* q_strides, int q_heads, void* q_out, const void* k, const long long* k_strides,
+                     int k_heads, void* k_out, int type, const float* cos_tab, const float* sin_tab, int table_len, int rotary_dim,
+                     int half_layout, int inverse, const long long* pos, long long pos_batch_stride, long long pos_token_stride,
+                     int batch, int tokens, int head_dim, ternaspmm_stream_t stream);
+
+/* The cache: codes uint8 [batch][kv_heads][max_len][head_dim / 2] and scales fp16 [batch][kv_heads][max_len][head_dim / 32] of keys
+ * and of values, 16-byte aligned; head_dim 64 or 128, max_len a multiple of 64.  A group of 32 values shares scale = fp16(m / -8), m its
+ * value of largest magnitude (the positive one of two); code = clamp(rint(x / scale) + 8, 0, 15) stands for scale * (code - 8).
+ * Codes are packed two a byte, the even one low; a key row then holds 4-byte word t of every group, t = 0 .. 3, a value row 2-byte
+ * halfword g of every group, g = 0 .. 7.
+ * start: int64 position of the first of `tokens` new tokens, of each sequence (start_stride 1) or of all (0); counts: int64 [batch],
+ * how many of them there are (null: all).  Sequences whose tokens do not fit into the cache are refused as a whole.
+ *
+ * _append: rotates q (may be null; then no q_out) and k by position where tables are given (bf16 results, ternaspmm_rotate's
+ * arithmetic) and writes the rows start .. start + count - 1.  8-byte aligned pointers, strides multiples of 4.
+ * _read: the values that rows stand for, bf16 [batch][tokens][kv_heads][head_dim]; zeros behind a sequence's count. */
+int ternaspmm_kv4_append(void* k_codes, void* k_scales, void* v_codes, void* v_scales, int max_len, const ternaspmm_bf16* k,
+                         const long long* k_strides, const ternaspmm_bf16* v, const long long* v_strides, const ternaspmm_bf16* q,
+                         const long long* q_strides, ternaspmm_bf16* q_out, const float* cos_tab, const float* sin_tab, int table_len,
+                         int rotary_dim, int half_layout, const long long* start, int start_stride, const long long* counts, int batch,
+                         int tokens, int heads, int kv_heads, int head_dim, ternaspmm_stream_t stream);
+int ternaspmm_kv4_read(void* k_codes, void* k_scales, void* v_codes, void* v_scales, int max_len, const long long* start,
+                       int start_stride, const long long* counts, ternaspmm_bf16* k_out, ternaspmm_bf16* v_out, int batch, int tokens,
+                       int kv_heads, int head_dim, ternaspmm_stream_t stream);
+
+/* Attention of the new tokens (already appended, queries already rotated) over the cache: the query of token t, at position p =
+ * start + t, sees the keys j <= p below start + count, with window > 0 only those above p - window.  A row that sees none is zero.
+ * scale: of the scores, > 0 and at most 1e6.  out bf16 [batch][tokens][heads][head_dim].  q, out 16-byte aligned, strides of q multiples of 8, heads
+ * a multiple of kv_heads.  workspace: ternaspmm_kv4_attend_workspace() bytes (may be 0; -1: shape not taken), 16-byte
+ * aligned, not shared by calls that may overlap on the GPU. */
+int ternaspmm_kv4_attend(const ternaspmm_bf16* q, const long long* q_strides, void* k_codes, void* k_scales, void* v_codes,
+                         void* v_scales, int max_len, const long long* start, int start_stride, const long long* counts, int window,
+                         float scale, ternaspmm_bf16* out, int batch, int tokens, int heads, int kv_heads, int head_dim, void* workspace,
+                         long long workspace_bytes, ternaspmm_stream_t stream);
+long long ternaspmm_kv4_attend_workspace(int batch, int tokens, int heads, int kv_heads, int head_dim, int max_len);
+
+/* Per row of logits [rows][vocab] (type as above, `ld` elements between rows): log probability of targets[row] (int64; negative: no
+ * token, 0), entropy, log of the sum of exponentials, and the `top` <= 32 most probable tokens with their log probabilities, the lowest id
+ * first among equal logits (NaN before all).  _grad: grad [rows][vocab] contiguous, of the logits' type, from the gradients of log probability
+ * and entropy (either may be null). */
+int ternaspmm_token_logprobs(const void* logits, long long ld, int type, const long long* targets, int rows, int vocab, int top,
+                             float* logprob, float* entropy, float* lse, float* top_logprob, long long* top_token,
+                             ternaspmm_stream_t stream);
+int ternaspmm_token_logprobs_grad(const void* logits, long long ld, int type, const long long* targets, int rows, int vocab,
+                                  const float* lse, const float* entropy, const float* g_logprob, const float* g_entropy, void* grad,
+                                  ternaspmm_stream_t stream);
+
 /* ---- work lists: many independent small-batch linears in one persistent launch ------------------
  * One item is what one call of bitlinear_TernaSpMM / ternaspmm_linear_segments /
  * bitlinear_TernaSpMM_residual computes, for 1 <= M <= 16 tokens.  A list runs all its items in ONE

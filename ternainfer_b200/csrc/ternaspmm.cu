@@ -22,9 +22,13 @@
 #include "attn_prefill.cuh"
 #include "dense_pair.cuh"
 #include "dense_prefill.cuh"
+#include "kv4.cuh"
+#include "kv4_attn.cuh"
 #include "lm_head.cuh"
+#include "logprobs.cuh"
 #include "mma_rate_probe.cuh"
 #include "pack_gpu.cuh"
+#include "rotary.cuh"
 #include "spmm_large_m.cuh"
 #include "spmm_list.cuh"
 #include "spmm_small_m.cuh"
@@ -1156,6 +1160,231 @@ extern "C" void ternaspmm_bf16_to_f32(__nv_bfloat16* x, float* y, long long n, c
     cudaLaunchConfig_t cfg = elementwise_launch(std::min<long long>((n + 15) / 16, 256ll * 8 * device_sm_count()), stream, &attr);
     if (cudaLaunchKernelEx(&cfg, bf16_to_f32_kernel, (const __nv_bfloat16*)x, y, n) != cudaSuccess) t_host_status = ST_LAUNCH;
     checkLastCudaError(__LINE__);
+}
+
+// ---- rotary positions (rotary.cuh) ------------------------------------------------------------------
+template <typename T, int V>
+static cudaError_t launch_rotate(const RotateParams& p, bool half, cudaStream_t stream) {
+    constexpr int HEADS = 4;
+    const int turned = half ? p.rotary / 2 / V : p.rotary / V, units = turned + (p.dim - p.rotary) / V;
+    const int head_groups = (p.q.heads + p.k.heads + HEADS - 1) / HEADS;
+    const long long items = p.tokens_all * head_groups * units;
+    if ((items + 255) / 256 > 0x7fffffffll) return cudaErrorInvalidValue;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((items + 255) / 256), 1, 1);
+    cfg.blockDim = dim3(256, 1, 1);
+    cfg.stream = stream;
+    if (half) return cudaLaunchKernelEx(&cfg, rotate_kernel<T, V, true, HEADS>, p, units, head_groups, items);
+    if constexpr (V > 1) return cudaLaunchKernelEx(&cfg, rotate_kernel<T, V, false, HEADS>, p, units, head_groups, items);
+    return cudaErrorInvalidValue;
+}
+
+template <typename T>
+static cudaError_t launch_rotate_type(const RotateParams& p, bool half, cudaStream_t stream) {
+    constexpr int V = 16 / sizeof(T);
+    // 16 bytes at a time where everything that a thread touches starts on such a boundary, else two elements (or one, in the half layout)
+    const long long steps = p.q.sb | p.q.st | p.q.sh | (p.k.heads ? p.k.sb | p.k.st | p.k.sh : 0) | (half ? p.rotary / 2 : p.rotary) | p.rotary | p.dim;
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(p.q.x) | reinterpret_cast<uintptr_t>(p.q.y) |
+                           (p.k.heads ? reinterpret_cast<uintptr_t>(p.k.x) | reinterpret_cast<uintptr_t>(p.k.y) : 0);
+    if (steps % V == 0 && bits % 16 == 0) return launch_rotate<T, V>(p, half, stream);
+    if (half) return launch_rotate<T, 1>(p, half, stream);
+    return steps % 2 == 0 && bits % (2 * sizeof(T)) == 0 ? launch_rotate<T, 2>(p, half, stream) : cudaErrorMisalignedAddress;
+}
+
+extern "C" int ternaspmm_rotate(const void* q, const long long* q_strides, int q_heads, void* q_out, const void* k, const long long* k_strides,
+                                int k_heads, void* k_out, int type, const float* cos_tab, const float* sin_tab, int table_len, int rotary_dim,
+                                int half_layout, int inverse, const long long* pos, long long pos_batch_stride, long long pos_token_stride,
+                                int batch, int tokens, int head_dim, cudaStream_t stream) {
+    t_host_status = ST_OK;
+    if (batch < 1 || tokens < 1 || q_heads < 1 || k_heads < 0 || head_dim < 2 || head_dim % 2 || rotary_dim < 2 || rotary_dim % 2 ||
+        rotary_dim > head_dim || table_len < 1 || type < 0 || type > 2)
+        return t_host_status = ST_BAD_SHAPE;
+    int* status = status_device_ptr();
+    const size_t size = type == 2 ? 4 : 2;
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(k_out);
+    if (!q || !q_strides || !q_out || (k_heads && (!k || !k_strides || !k_out)) || !cos_tab || !sin_tab || !pos || bits % size)
+        return t_host_status = ST_BAD_POINTER;
+    if (!status) return t_host_status = ST_LAUNCH;
+    RotateParams p = {};
+    p.q = {q, q_out, q_strides[0], q_strides[1], q_strides[2], q_heads};
+    if (k_heads) p.k = {k, k_out, k_strides[0], k_strides[1], k_strides[2], k_heads};
+    p.cos_tab = cos_tab, p.sin_tab = sin_tab, p.pos = pos, p.pos_sb = pos_batch_stride, p.pos_st = pos_token_stride;
+    p.tokens_all = (long long)batch * tokens, p.tokens = tokens, p.dim = head_dim, p.rotary = rotary_dim, p.table_len = table_len;
+    p.sign = inverse ? -1.f : 1.f, p.status = status;
+    const cudaError_t e = type == 0 ? launch_rotate_type<__nv_bfloat16>(p, half_layout != 0, stream)
+                          : type == 1 ? launch_rotate_type<__half>(p, half_layout != 0, stream) : launch_rotate_type<float>(p, half_layout != 0, stream);
+    if (e == cudaErrorMisalignedAddress) return t_host_status = ST_BAD_POINTER;
+    if (e != cudaSuccess) t_host_status = ST_LAUNCH;
+    checkLastCudaError(__LINE__);
+    return t_host_status;
+}
+
+// ---- key / value cache in 4 bits (kv4.cuh, kv4_attn.cuh) ----------------------------------------------
+static bool kv4_cache(Kv4Cache& c, void* k_codes, void* k_scales, void* v_codes, void* v_scales, int kv_heads, int max_len) {
+    c = {static_cast<uint8_t*>(k_codes), static_cast<uint8_t*>(v_codes), static_cast<__half*>(k_scales), static_cast<__half*>(v_scales), kv_heads, max_len};
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(k_codes) | reinterpret_cast<uintptr_t>(k_scales) | reinterpret_cast<uintptr_t>(v_codes) |
+                           reinterpret_cast<uintptr_t>(v_scales);
+    return k_codes && k_scales && v_codes && v_scales && !(bits & 15);
+}
+static bool kv4_shape(int batch, int tokens, int kv_heads, int head_dim, int max_len) {
+    return batch >= 1 && batch <= 65535 && tokens >= 1 && kv_heads >= 1 && (head_dim == 64 || head_dim == 128) && max_len >= kKv4Tile &&
+           max_len % kKv4Tile == 0 && max_len <= (1 << 30);
+}
+// 2 values of bf16 at a time: every row starts on 8 bytes
+static bool kv4_side(Kv4Side& s, const __nv_bfloat16* x, const long long* strides, int align) {
+    if (!x || !strides || (reinterpret_cast<uintptr_t>(x) & (align - 1)) || ((strides[0] | strides[1] | strides[2]) & (align / 2 - 1))) return false;
+    s = {x, strides[0], strides[1], strides[2]};
+    return true;
+}
+
+extern "C" int ternaspmm_kv4_append(void* k_codes, void* k_scales, void* v_codes, void* v_scales, int max_len, const __nv_bfloat16* k,
+                                    const long long* k_strides, const __nv_bfloat16* v, const long long* v_strides, const __nv_bfloat16* q,
+                                    const long long* q_strides, __nv_bfloat16* q_out, const float* cos_tab, const float* sin_tab, int table_len,
+                                    int rotary_dim, int half_layout, const long long* start, int start_stride, const long long* counts, int batch,
+                                    int tokens, int heads, int kv_heads, int head_dim, cudaStream_t stream) {
+    t_host_status = ST_OK;
+    if (!kv4_shape(batch, tokens, kv_heads, head_dim, max_len) || (q && heads < 1) ||
+        (cos_tab && (rotary_dim < 2 || rotary_dim % 2 || rotary_dim > head_dim || table_len < 1)))
+        return t_host_status = ST_BAD_SHAPE;
+    Kv4AppendParams p = {};
+    p.status = status_device_ptr();
+    if (!kv4_cache(p.c, k_codes, k_scales, v_codes, v_scales, kv_heads, max_len) || !kv4_side(p.k, k, k_strides, 8) || !kv4_side(p.v, v, v_strides, 8) ||
+        (q && (!kv4_side(p.q, q, q_strides, 8) || !q_out || (reinterpret_cast<uintptr_t>(q_out) & 7) || !cos_tab)) || (!cos_tab != !sin_tab) || !start)
+        return t_host_status = ST_BAD_POINTER;
+    p.q_out = q_out, p.cos_tab = cos_tab, p.sin_tab = sin_tab, p.start = start, p.counts = counts, p.start_stride = start_stride ? 1 : 0;
+    p.tokens = tokens, p.heads = q ? heads : 0, p.rotary = rotary_dim, p.half = half_layout != 0, p.table_len = table_len;
+    const long long rows = (long long)batch * tokens * (p.heads + 2ll * kv_heads), blocks = (rows * (head_dim / 4) + 255) / 256;
+    if (!p.status || blocks > 0x7fffffffll) return t_host_status = !p.status ? ST_LAUNCH : ST_BAD_SHAPE;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks, 1, 1);
+    cfg.blockDim = dim3(256, 1, 1);
+    cfg.stream = stream;
+    if (cudaLaunchKernelEx(&cfg, head_dim == 128 ? kv4_append_kernel<128> : kv4_append_kernel<64>, p, rows) != cudaSuccess) t_host_status = ST_LAUNCH;
+    checkLastCudaError(__LINE__);
+    return t_host_status;
+}
+
+extern "C" int ternaspmm_kv4_read(void* k_codes, void* k_scales, void* v_codes, void* v_scales, int max_len, const long long* start, int start_stride,
+                                  const long long* counts, __nv_bfloat16* k_out, __nv_bfloat16* v_out, int batch, int tokens, int kv_heads, int head_dim,
+                                  cudaStream_t stream) {
+    t_host_status = ST_OK;
+    if (!kv4_shape(batch, tokens, kv_heads, head_dim, max_len)) return t_host_status = ST_BAD_SHAPE;
+    Kv4ReadParams p = {};
+    p.status = status_device_ptr();
+    if (!kv4_cache(p.c, k_codes, k_scales, v_codes, v_scales, kv_heads, max_len) || !start || !k_out || !v_out ||
+        ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 7))
+        return t_host_status = ST_BAD_POINTER;
+    p.k_out = k_out, p.v_out = v_out, p.start = start, p.counts = counts, p.start_stride = start_stride ? 1 : 0, p.tokens = tokens;
+    const long long rows = (long long)batch * tokens * 2 * kv_heads, blocks = (rows * (head_dim / 4) + 255) / 256;
+    if (!p.status || blocks > 0x7fffffffll) return t_host_status = !p.status ? ST_LAUNCH : ST_BAD_SHAPE;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks, 1, 1);
+    cfg.blockDim = dim3(256, 1, 1);
+    cfg.stream = stream;
+    if (cudaLaunchKernelEx(&cfg, head_dim == 128 ? kv4_read_kernel<128> : kv4_read_kernel<64>, p, rows) != cudaSuccess) t_host_status = ST_LAUNCH;
+    checkLastCudaError(__LINE__);
+    return t_host_status;
+}
+
+// How an attention call is cut: rows per CTA, tiles of rows per key / value head, splits over the keys.
+struct Kv4Plan {
+    int rows, row_tiles, splits;
+};
+static Kv4Plan kv4_plan(int batch, int tokens, int heads, int kv_heads, int max_len) {
+    const long long rows_all = (long long)tokens * (heads / kv_heads);
+    Kv4Plan pl;
+    pl.rows = rows_all <= 8 ? 8 : 16;
+    pl.row_tiles = (int)((rows_all + pl.rows - 1) / pl.rows);
+    const long long items = (long long)batch * kv_heads * pl.row_tiles;
+    const long long want = (3ll * device_sm_count() + items - 1) / items, most = (max_len / 16 + kKv4Warps - 1) / kKv4Warps;
+    pl.splits = (int)std::max<long long>(1, std::min(want, most));
+    return pl;
+}
+static bool kv4_attend_shape(int batch, int tokens, int heads, int kv_heads, int head_dim, int max_len) {
+    return kv4_shape(batch, tokens, kv_heads, head_dim, max_len) && heads >= kv_heads && heads % kv_heads == 0 && (long long)tokens * heads < (1ll << 30);
+}
+
+extern "C" long long ternaspmm_kv4_attend_workspace(int batch, int tokens, int heads, int kv_heads, int head_dim, int max_len) {
+    if (!kv4_attend_shape(batch, tokens, heads, kv_heads, head_dim, max_len)) return -1;
+    const Kv4Plan pl = kv4_plan(batch, tokens, heads, kv_heads, max_len);
+    return pl.splits == 1 ? 0 : (long long)batch * kv_heads * pl.row_tiles * pl.splits * pl.rows * (head_dim + 2) * 4;
+}
+
+template <int D, int ROWS>
+static cudaError_t launch_kv4_attend(const Kv4AttnParams& p, int batch, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(p.splits * p.row_tiles * p.c.kv_heads), batch, 1);
+    cfg.blockDim = dim3(kKv4Warps * 32, 1, 1);
+    cfg.stream = stream;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kv4_attn_kernel<D, ROWS>, p);
+    if (e != cudaSuccess || p.splits == 1) return e;
+    cfg.gridDim = dim3((unsigned)(ROWS * p.row_tiles * p.c.kv_heads), batch, 1);
+    cfg.blockDim = dim3(D, 1, 1);
+    return cudaLaunchKernelEx(&cfg, kv4_attn_join_kernel<D, ROWS>, p);
+}
+
+extern "C" int ternaspmm_kv4_attend(const __nv_bfloat16* q, const long long* q_strides, void* k_codes, void* k_scales, void* v_codes, void* v_scales,
+                                    int max_len, const long long* start, int start_stride, const long long* counts, int window, float scale,
+                                    __nv_bfloat16* out, int batch, int tokens, int heads, int kv_heads, int head_dim, void* workspace,
+                                    long long workspace_bytes, cudaStream_t stream) {
+    t_host_status = ST_OK;
+    const long long need = ternaspmm_kv4_attend_workspace(batch, tokens, heads, kv_heads, head_dim, max_len);
+    if (need < 0 || window < 0 || !(scale > 0.f) || scale > 1e6f || workspace_bytes < need) return t_host_status = ST_BAD_SHAPE;
+    Kv4AttnParams p = {};
+    p.status = status_device_ptr();
+    if (!kv4_cache(p.c, k_codes, k_scales, v_codes, v_scales, kv_heads, max_len) || !kv4_side(p.q, q, q_strides, 16) || !start || !out ||
+        (reinterpret_cast<uintptr_t>(out) & 15) || (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15))))
+        return t_host_status = ST_BAD_POINTER;
+    if (!p.status) return t_host_status = ST_LAUNCH;
+    const Kv4Plan pl = kv4_plan(batch, tokens, heads, kv_heads, max_len);
+    p.start = start, p.counts = counts, p.start_stride = start_stride ? 1 : 0, p.out = out, p.tokens = tokens, p.heads = heads, p.window = window;
+    p.splits = pl.splits, p.row_tiles = pl.row_tiles, p.scale_log2 = scale * 1.4426950408889634f;
+    p.part_o = static_cast<float*>(workspace);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + (size_t)batch * kv_heads * pl.row_tiles * pl.splits * pl.rows * head_dim);
+    const cudaError_t e = head_dim == 128 ? (pl.rows == 8 ? launch_kv4_attend<128, 8>(p, batch, stream) : launch_kv4_attend<128, 16>(p, batch, stream))
+                                          : (pl.rows == 8 ? launch_kv4_attend<64, 8>(p, batch, stream) : launch_kv4_attend<64, 16>(p, batch, stream));
+    if (e != cudaSuccess) t_host_status = ST_LAUNCH;
+    checkLastCudaError(__LINE__);
+    return t_host_status;
+}
+
+// ---- log probabilities of given tokens (logprobs.cuh) -------------------------------------------------
+extern "C" int ternaspmm_token_logprobs(const void* logits, long long ld, int type, const long long* targets, int rows, int vocab, int top,
+                                        float* logprob, float* entropy, float* lse, float* top_logprob, long long* top_token, cudaStream_t stream) {
+    t_host_status = ST_OK;
+    if (rows < 1 || vocab < 1 || ld < vocab || type < 0 || type > 2 || top < 0 || top > kLpMaxTop || top > vocab) return t_host_status = ST_BAD_SHAPE;
+    LogprobParams p = {logits, ld, targets, logprob, entropy, lse, top_logprob, top_token, vocab, top, status_device_ptr()};
+    if (!logits || !targets || !logprob || !entropy || !lse || (top && (!top_logprob || !top_token)) || reinterpret_cast<uintptr_t>(logits) % (type == 2 ? 4 : 2))
+        return t_host_status = ST_BAD_POINTER;
+    if (!p.status) return t_host_status = ST_LAUNCH;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)rows, 1, 1);
+    cfg.blockDim = dim3(kLpThreads, 1, 1);
+    cfg.stream = stream;
+    if (cudaLaunchKernelEx(&cfg, type == 0 ? logprob_kernel<__nv_bfloat16> : type == 1 ? logprob_kernel<__half> : logprob_kernel<float>, p) != cudaSuccess)
+        t_host_status = ST_LAUNCH;
+    checkLastCudaError(__LINE__);
+    return t_host_status;
+}
+
+extern "C" int ternaspmm_token_logprobs_grad(const void* logits, long long ld, int type, const long long* targets, int rows, int vocab,
+                                             const float* lse, const float* entropy, const float* g_logprob, const float* g_entropy, void* grad,
+                                             cudaStream_t stream) {
+    t_host_status = ST_OK;
+    if (rows < 1 || vocab < 1 || ld < vocab || type < 0 || type > 2) return t_host_status = ST_BAD_SHAPE;
+    if (!logits || !targets || !lse || !entropy || !grad || (reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(grad)) % (type == 2 ? 4 : 2))
+        return t_host_status = ST_BAD_POINTER;
+    LogprobGradParams p = {logits, ld, targets, lse, entropy, g_logprob, g_entropy, grad, vocab};
+    const int parts = (vocab + 8191) / 8192;
+    if ((long long)rows * parts > 0x7fffffffll) return t_host_status = ST_BAD_SHAPE;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((long long)rows * parts), 1, 1);
+    cfg.blockDim = dim3(256, 1, 1);
+    cfg.stream = stream;
+    if (cudaLaunchKernelEx(&cfg, type == 0 ? logprob_grad_kernel<__nv_bfloat16> : type == 1 ? logprob_grad_kernel<__half> : logprob_grad_kernel<float>, p, parts) != cudaSuccess)
+        t_host_status = ST_LAUNCH;
+    checkLastCudaError(__LINE__);
+    return t_host_status;
 }
 
 extern "C" void ternaspmm_partial_f32(int8_t* x, uint64_t* bitmap, int* tile_offsets, uint16_t* quarter_offsets,

@@ -1,0 +1,171 @@
+"""Rotary positions: tables of the angles and the kernel that turns queries and keys by them.
+
+``linear.rope`` and the attention kernels rotate adjacent pairs of a whole head of 128 by the reference's unscaled angles
+(model.py:205-243 of Gu-J/TernaInfer).  Here are the other forms that checkpoints are trained with: pairs of the two halves, a
+part of the head, and angles scaled for contexts longer than the trained ones.  Kernel: csrc/rotary.cuh.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from .lib import load_library
+from .linear import _on, _stream
+
+LAYOUTS = ("interleaved", "half")
+_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+@dataclass(frozen=True)
+class RotaryTable:
+    """cos, sin: fp32 [max_len, rotary_dim / 2], contiguous, on one device; pairs (2i, 2i+1) of a head's first rotary_dim values
+    ("interleaved") or (i, i + rotary_dim / 2) ("half")."""
+    cos: torch.Tensor
+    sin: torch.Tensor
+    layout: str = "interleaved"
+
+    def __post_init__(self):
+        if self.layout not in LAYOUTS:
+            raise ValueError(f"layout is one of {LAYOUTS}, not {self.layout!r}")
+        for t in (self.cos, self.sin):
+            if t.dtype != torch.float32 or t.dim() != 2 or t.shape != self.cos.shape or not t.is_contiguous() or t.numel() == 0 or t.device != self.cos.device:
+                raise ValueError("cos and sin are contiguous fp32 tensors [max_len, rotary_dim / 2] of one device")
+
+    @property
+    def rotary_dim(self) -> int:
+        return 2 * self.cos.shape[1]
+
+    @property
+    def max_len(self) -> int:
+        return self.cos.shape[0]
+
+
+def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: Optional[dict] = None, device="cpu"):
+    """(angle per position of every pair, float64 [rotary_dim / 2]; factor of cosines and sines).  ``scaling``:
+    None, or a dict with "type" and "factor" (how many times longer the context is than the trained one):
+      linear      every angle divided by factor
+      ntk         theta raised so that the slowest pair turns `factor` times slower and the fastest as before
+      yarn        pairs that turn more than beta_fast (32) times over original_len as before, those with fewer than beta_slow (1) turns divided
+                  by factor, a ramp over the pairs between; cosines and sines times 0.1 ln(factor) + 1
+      wavelength  pairs with more than `high` (4) turns over original_len as before, those with fewer than `low` (1) divided by factor,
+                  mixed by their number of turns between."""
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim is even and at least 2, not {rotary_dim}")
+    pair = torch.arange(rotary_dim // 2, dtype=torch.float64, device=device)
+    inv = theta ** (-2 * pair / rotary_dim)
+    if scaling is None:
+        return inv, 1.0
+    kind, factor = scaling.get("type"), float(scaling.get("factor", 0))
+    known = {"linear": (), "ntk": (), "yarn": ("original_len", "beta_fast", "beta_slow"), "wavelength": ("original_len", "low", "high")}
+    if kind not in known or not factor > 0:
+        raise ValueError(f"scaling has a type of {tuple(known)} and a factor above 0: {scaling}")
+    if extra := set(scaling) - {"type", "factor", *known[kind]}:
+        raise ValueError(f"{kind} scaling does not know {sorted(extra)}")
+    if kind == "linear":
+        return inv / factor, 1.0
+    if kind == "ntk":
+        if rotary_dim == 2:
+            raise ValueError("ntk scaling needs a rotary_dim above 2")
+        return (theta * factor ** (rotary_dim / (rotary_dim - 2))) ** (-2 * pair / rotary_dim), 1.0
+    if "original_len" not in scaling:
+        raise ValueError(f"{kind} scaling needs original_len")
+    length = float(scaling["original_len"])
+    if kind == "yarn":
+        fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
+
+        def pair_with(turns):                # index of the pair that turns so often over the original length
+            return rotary_dim * math.log(length / (2 * math.pi * turns)) / (2 * math.log(theta))
+        lo, hi = max(math.floor(pair_with(fast)), 0), min(math.ceil(pair_with(slow)), rotary_dim - 1)
+        ramp = ((pair - lo) / max(hi - lo, 0.001)).clamp(0, 1)
+        return inv / factor * ramp + inv * (1 - ramp), 0.1 * math.log(factor) + 1 if factor > 1 else 1.0
+    low, high = float(scaling.get("low", 1.0)), float(scaling.get("high", 4.0))
+    if not high > low:
+        raise ValueError("wavelength scaling needs high > low")
+    keep = ((length * inv / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
+    return inv * keep + inv / factor * (1 - keep), 1.0
+
+
+def rotary_table(head_dim: int, max_len: int, theta: float = 10000.0, *, rotary_dim: Optional[int] = None, layout: str = "interleaved",
+                 scaling: Optional[dict] = None, device="cuda") -> RotaryTable:
+    """Cosines and sines of positions 0 .. max_len - 1, computed in 64 bits (an fp32 angle of position 131072 is off by 0.004).
+    ``rotary_dim``: how much of a head is rotated (all of it)."""
+    rotary_dim = head_dim if rotary_dim is None else rotary_dim
+    if rotary_dim > head_dim or max_len < 1:
+        raise ValueError(f"rotary_dim {rotary_dim} of a head of {head_dim}, {max_len} positions")
+    inv, factor = rotary_frequencies(rotary_dim, theta, scaling, device)
+    angle = torch.arange(max_len, dtype=torch.float64, device=device)[:, None] * inv
+    return RotaryTable((angle.cos() * factor).float(), (angle.sin() * factor).float(), layout)
+
+
+def _strides(t: torch.Tensor):
+    return (ctypes.c_longlong * 3)(*t.stride()[:3])
+
+
+def _takes(x: torch.Tensor, layout: str):
+    """x as the kernel reads it: contiguous heads, whole pairs on their boundaries in the interleaved layout."""
+    if x.stride(3) != 1 or (layout == "interleaved" and (any(s % 2 for s in x.stride()[:3]) or x.data_ptr() % (2 * x.element_size()))):
+        return x.contiguous()
+    return x
+
+
+def _launch(q, k, table, positions, inverse):
+    B, T, H, D = q.shape
+    q, k = _takes(q, table.layout), None if k is None else _takes(k, table.layout)
+    out = torch.empty((B, T, H, D), dtype=q.dtype, device=q.device)
+    k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    if q.numel() == 0:
+        return out, k_out
+    shared = positions.dim() == 1
+    with _on(q):
+        status = load_library().ternaspmm_rotate(
+            q.data_ptr(), _strides(q), H, out.data_ptr(), None if k is None else k.data_ptr(), None if k is None else _strides(k),
+            0 if k is None else k.shape[2], None if k is None else k_out.data_ptr(), _TYPES[q.dtype], table.cos.data_ptr(), table.sin.data_ptr(),
+            table.max_len, table.rotary_dim, table.layout == "half", inverse, positions.data_ptr(), 0 if shared else positions.stride(0),
+            positions.stride(-1), B, T, D, _stream())
+    if status:
+        raise RuntimeError(f"ternaspmm_rotate: status {status}")
+    return out, k_out
+
+
+class _Rotate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, cos, sin, layout, positions):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(cos, sin, positions)
+        ctx.layout = layout
+        return _launch(q, k, RotaryTable(cos, sin, layout), positions, False)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gq, gk):
+        cos, sin, positions = ctx.saved_tensors
+        table = RotaryTable(cos, sin, ctx.layout)
+        gq, gk = (g if need else None for g, need in zip((gq, gk), ctx.needs_input_grad))
+        if gq is not None:
+            gq, gk = _launch(gq, gk, table, positions, True)
+        elif gk is not None:
+            gk = _launch(gk, None, table, positions, True)[0]
+        return gq, gk, None, None, None, None
+
+
+def rotate(q: torch.Tensor, k: Optional[torch.Tensor], table: RotaryTable, positions: torch.Tensor):
+    """Queries [B, T, H, D] and keys [B, T, Hkv, D] (or None) turned by the angles of their positions, in one launch: (q, k) of the same type
+    (bf16, fp16 or fp32), products in fp32, rounded once.  ``positions``: int64 [T] or [B, T] on the device.  Strided views are taken as
+    they are.  Differentiable in q and k.  A position outside of the table gives NaN in its token and status 1 of the library."""
+    if not q.is_cuda:
+        raise RuntimeError("rotate needs CUDA tensors: the B200 library has no CPU path")
+    if q.dim() != 4 or q.dtype not in _TYPES or q.shape[3] % 2:
+        raise ValueError(f"q is bf16, fp16 or fp32 [B, T, H, D] with an even D, not {q.dtype} {list(q.shape)}")
+    if k is not None and (k.dim() != 4 or k.dtype != q.dtype or k.device != q.device or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3]):
+        raise ValueError(f"k is {q.dtype} [B, T, Hkv, D] beside q, not {k.dtype} {list(k.shape)}")
+    if positions.dtype != torch.int64 or positions.device != q.device or list(positions.shape) not in ([q.shape[1]], list(q.shape[:2])):
+        raise ValueError(f"positions are int64 [T] or [B, T] on {q.device}, not {positions.dtype} {list(positions.shape)}")
+    if table.rotary_dim > q.shape[3] or table.cos.device != q.device:
+        raise ValueError(f"the table rotates {table.rotary_dim} values on {table.cos.device}, a head has {q.shape[3]} on {q.device}")
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _Rotate.apply(q, k, table.cos, table.sin, table.layout, positions)
+    return _launch(q, k, table, positions, False)

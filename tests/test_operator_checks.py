@@ -1,0 +1,102 @@
+"""CPU: what the rotary, 4-bit cache and scoring operators refuse before anything is launched, and the frequencies of scaled rotations."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from ternainfer_b200.kv4 import KV4Cache, kv4_append, kv4_attend, kv4_read
+from ternainfer_b200.rotary import RotaryTable, rotary_frequencies, rotary_table, rotate
+from ternainfer_b200.scores import token_logprobs
+
+P = 1 << 20                     # an aligned address that nothing reads: every call below is refused on the host
+
+
+def strides(*v):
+    return (ctypes.c_longlong * 3)(*v)
+
+
+def test_cpu_tensors_are_refused():
+    x, pos = torch.zeros((1, 2, 1, 64), dtype=torch.bfloat16), torch.zeros(2, dtype=torch.int64)
+    table, cache = rotary_table(64, 8, device="cpu"), KV4Cache.empty(1, 1, 64, 64, device="cpu")
+    for call in (lambda: rotate(x, None, table, pos), lambda: kv4_append(cache, x, x, pos[:1]), lambda: kv4_read(cache, pos[:1], 2),
+                 lambda: kv4_attend(x, cache, pos[:1]), lambda: token_logprobs(torch.zeros((2, 5)), pos)):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            call()
+
+
+def test_cache_shapes():
+    c = KV4Cache.empty(2, 3, 100, 128, device="cpu")
+    assert (c.batch, c.kv_heads, c.max_len, c.head_dim) == (2, 3, 128, 128)
+    assert c.k_codes.shape == (2, 3, 128, 64) and c.v_scales.shape == (2, 3, 128, 4)
+    for bad in ((c.k_codes.float(), c.k_scales, c.v_codes, c.v_scales), (c.k_codes, c.k_scales[..., :2], c.v_codes, c.v_scales),
+                (c.k_codes, c.k_scales, c.v_codes.transpose(1, 2), c.v_scales)):
+        with pytest.raises(ValueError):
+            KV4Cache(*bad)
+
+
+def test_frequencies():
+    theta, n = 10000.0, 32
+    plain, one = rotary_frequencies(n, theta)
+    assert one == 1 and torch.equal(plain, theta ** (-torch.arange(0, n, 2, dtype=torch.float64) / n))
+    assert torch.equal(rotary_frequencies(n, theta, dict(type="linear", factor=3))[0], plain / 3)
+    ntk = rotary_frequencies(n, theta, dict(type="ntk", factor=3))[0]
+    assert ntk[0] == plain[0] and abs(ntk[-1] * 3 / plain[-1] - 1) < 1e-12
+    for scaling in (dict(type="yarn", factor=5, original_len=4096), dict(type="wavelength", factor=5, original_len=4096)):
+        inv, size = rotary_frequencies(n, theta, scaling)
+        turns = 4096 * plain / (2 * math.pi)
+        ratio = plain / inv
+        assert (ratio[turns > 32] == 1).all() and (abs(ratio[turns < 1] - 5) < 1e-12).all() and (ratio[1:] >= ratio[:-1]).all() and 1 < ratio[(turns > 3) & (turns < 4)].min()
+        assert size == (0.1 * math.log(5) + 1 if scaling["type"] == "yarn" else 1)
+    for bad in (dict(type="other", factor=2), dict(type="linear"), dict(type="linear", factor=-1), dict(type="linear", factor=2, low=3), dict(type="yarn", factor=2),
+                dict(type="wavelength", factor=2, original_len=9, low=4, high=4)):
+        with pytest.raises(ValueError):
+            rotary_frequencies(n, theta, bad)
+    for bad in (0, 1, 7):
+        with pytest.raises(ValueError):
+            rotary_frequencies(bad)
+    with pytest.raises(ValueError):
+        rotary_table(64, 8, rotary_dim=128, device="cpu")
+    with pytest.raises(ValueError):
+        RotaryTable(torch.zeros(3, 4), torch.zeros(3, 4), "other")
+
+
+def test_rotate_statuses(lib):
+    good = dict(q=P, qs=strides(64, 64, 64), qh=1, qo=P, k=None, ks=None, kh=0, ko=None, type=0, cos=P, sin=P, len=4, rot=64, half=0, inv=0, pos=P, sb=0, st=1,
+                batch=1, tokens=1, dim=64)
+    for status, change in ((1, dict(batch=0)), (1, dict(tokens=0)), (1, dict(qh=0)), (1, dict(kh=-1)), (1, dict(dim=63)), (1, dict(rot=66)), (1, dict(rot=7)),
+                           (1, dict(len=0)), (1, dict(type=3)), (2, dict(q=None)), (2, dict(qo=None)), (2, dict(kh=1)), (2, dict(cos=None)), (2, dict(pos=None)),
+                           (2, dict(q=P + 1)), (2, dict(qs=None))):
+        assert lib.ternaspmm_rotate(*{**good, **change}.values(), None) == status, change
+        assert lib.ternaspmm_last_status() == status
+
+
+def test_kv4_statuses(lib):
+    s = strides(64, 64, 64)
+    append = dict(kc=P, ks=P, vc=P, vs=P, L=64, k=P, kst=s, v=P, vst=s, q=None, qst=None, qo=None, cos=None, sin=None, len=0, rot=0, half=0, start=P, ss=1, counts=None,
+                  batch=1, tokens=1, heads=0, kv=1, dim=64)
+    for status, change in ((1, dict(batch=0)), (1, dict(batch=65536)), (1, dict(tokens=0)), (1, dict(kv=0)), (1, dict(dim=96)), (1, dict(L=0)), (1, dict(L=100)),
+                           (1, dict(cos=P, sin=P, rot=66, len=4)), (1, dict(q=P, heads=0)), (2, dict(kc=None)), (2, dict(vs=P + 8)), (2, dict(k=None)),
+                           (2, dict(k=P + 2)), (2, dict(vst=strides(64, 64, 2))), (2, dict(start=None)), (2, dict(cos=P, rot=64, len=4)),
+                           (2, dict(q=P, qst=s, qo=P, heads=1)), (2, dict(q=P, qst=s, heads=1, cos=P, sin=P, rot=64, len=4))):
+        assert lib.ternaspmm_kv4_append(*{**append, **change}.values(), None) == status, change
+    read = dict(kc=P, ks=P, vc=P, vs=P, L=64, start=P, ss=1, counts=None, k=P, v=P, batch=1, tokens=1, kv=1, dim=64)
+    for status, change in ((1, dict(L=96)), (1, dict(tokens=-1)), (2, dict(k=None)), (2, dict(v=P + 4)), (2, dict(start=None))):
+        assert lib.ternaspmm_kv4_read(*{**read, **change}.values(), None) == status, change
+    attend = dict(q=P, qst=s, kc=P, ks=P, vc=P, vs=P, L=64, start=P, ss=1, counts=None, window=0, scale=0.125, out=P, batch=1, tokens=1, heads=2, kv=1, dim=64, ws=P,
+                  bytes=1 << 40)
+    for status, change in ((1, dict(heads=3, kv=2)), (1, dict(heads=0)), (1, dict(window=-1)), (1, dict(scale=0.0)), (1, dict(scale=math.nan)), (1, dict(scale=math.inf)),
+                           (1, dict(bytes=-1)), (1, dict(dim=32)), (1, dict(tokens=1 << 30)), (2, dict(q=P + 8)), (2, dict(qst=strides(64, 64, 4))), (2, dict(out=None)),
+                           (2, dict(ks=None))):
+        assert lib.ternaspmm_kv4_attend(*{**attend, **change}.values(), None) == status, change
+    assert lib.ternaspmm_kv4_attend_workspace(1, 1, 3, 2, 64, 64) == -1 and lib.ternaspmm_kv4_attend_workspace(1, 1, 4, 2, 64, 1 << 20) >= 0
+
+
+def test_logprob_statuses(lib):
+    good = dict(x=P, ld=10, type=0, t=P, rows=1, vocab=10, top=2, lp=P, h=P, lse=P, tl=P, tt=P)
+    for status, change in ((1, dict(rows=0)), (1, dict(vocab=0)), (1, dict(ld=9)), (1, dict(type=-1)), (1, dict(top=33, vocab=50, ld=50)), (1, dict(top=11)), (1, dict(top=-1)),
+                           (2, dict(x=None)), (2, dict(x=P + 1)), (2, dict(t=None)), (2, dict(lse=None)), (2, dict(tt=None))):
+        assert lib.ternaspmm_token_logprobs(*{**good, **change}.values(), None) == status, change
+    grad = dict(x=P, ld=10, type=2, t=P, rows=1, vocab=10, lse=P, h=P, gl=None, gh=P, out=P)
+    for status, change in ((1, dict(rows=0)), (1, dict(ld=9)), (2, dict(out=P + 2)), (2, dict(h=None))):
+        assert lib.ternaspmm_token_logprobs_grad(*{**grad, **change}.values(), None) == status, change
