@@ -117,8 +117,13 @@ def main():
     ap.add_argument("--no_cuda_graph", action="store_true")
     ap.add_argument("--seed", type=int, default=1234)
     ap.add_argument("--fused_glue", action="store_true", help="fused norm+quantiser kernels, residual add in the epilogue")
+    ap.add_argument("--kv_bits", type=int, default=16, choices=(16, 4), help="4: keys and values in a 4-bit cache")
+    ap.add_argument("--rope_layout", default="interleaved", choices=("interleaved", "half"))
+    ap.add_argument("--rope_linear", type=float, default=1.0, help="positions divided by this, for contexts longer than the trained one")
+    ap.add_argument("--top_logprobs", type=int, default=0, help="score prompt and generated tokens, with this many alternatives")
     a = ap.parse_args()
-    margs = ModelArgs(n_layers=a.layers, fused_glue=a.fused_glue)
+    margs = ModelArgs(n_layers=a.layers, fused_glue=a.fused_glue, kv_bits=a.kv_bits, rope_layout=a.rope_layout,
+                      rope_scaling=dict(type="linear", factor=a.rope_linear) if a.rope_linear != 1 else None)
     model, _ = build_random_model(margs, a.prompt_length + a.gen_length, a.seed)
     gen = FastGen(model, GenArgs(a.gen_length, a.bsz, a.prompt_length, not a.no_cuda_graph))
     g = torch.Generator(device="cuda").manual_seed(a.seed + 1)
@@ -126,6 +131,12 @@ def main():
     gen.generate(prompt)            # warm-up (captures the graphs)
     tokens, stats = gen.generate(prompt)
     print({k: round(v, 4) for k, v in stats.items()}, "first tokens", tokens[0, :8].tolist())
+    if a.top_logprobs:
+        with torch.inference_mode():
+            r = model.score(torch.cat([prompt, tokens], 1), gen.cache, top=a.top_logprobs)
+        n = a.gen_length
+        print("log probability per generated token %.4f, entropy %.4f, most probable %s" % (
+            r.logprob[:, -n:].mean().item(), r.entropy[:, -n:].mean().item(), r.top_token[0, -n].tolist()))
 
 
 if __name__ == "__main__":

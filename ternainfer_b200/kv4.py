@@ -69,6 +69,8 @@ class KV4Cache:
 def _check(cache: KV4Cache, name: str, x: Optional[torch.Tensor], heads: Optional[int]):
     if not x.is_cuda:
         raise RuntimeError(f"{name} needs CUDA tensors: the B200 library has no CPU path")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name} requires a gradient: the 4-bit cache has none")
     if (x.dim() != 4 or x.dtype != torch.bfloat16 or x.device != cache.k_codes.device or x.shape[0] != cache.batch or x.shape[3] != cache.head_dim
             or x.shape[2] == 0 or (heads is not None and x.shape[2] != heads)):
         raise ValueError(f"{name}: bf16 [{cache.batch}, T, {heads or 'heads'}, {cache.head_dim}] on {cache.k_codes.device} wanted, not {x.dtype} {list(x.shape)} on {x.device}")

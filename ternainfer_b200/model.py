@@ -20,7 +20,10 @@ import torch
 from torch import nn
 from torch.nn import functional as F
 
+from .kv4 import KV4Cache, kv4_append, kv4_attend
 from .linear import SpBitLinear, attn_decode, attn_decode_by_head, attn_prefill, lm_head_argmax, quant_input, relu2_gate, rmsnorm, rope, to_float
+from .rotary import LAYOUTS, rotary_table, rotate
+from .scores import TokenLogprobs, token_logprobs
 
 
 @dataclass
@@ -36,6 +39,10 @@ class ModelArgs:
     use_kernel: bool = True
     fused_glue: bool = False     # fused norm+quantiser kernels and residual add in the linear epilogue
     flash_attention: Optional[bool] = None   # attention glue through flash_attn's kv-cache kernel; None = with fused_glue
+    kv_bits: int = 16            # 4: keys and values in a 4-bit cache (kv4.py)
+    rope_layout: str = "interleaved"         # or "half"
+    rotary_dim: Optional[int] = None         # how much of a head is rotated (all of it)
+    rope_scaling: Optional[dict] = None      # rotary.rotary_frequencies
 
     @property
     def head_dim(self) -> int:
@@ -119,9 +126,20 @@ class Attention(nn.Module):
             with torch.no_grad():
                 self.attn_sub_norm.weight.copy_(dic[prefix + ".attn_sub_norm.weight"])
 
-    def forward(self, x, cache: LayerCache, pos, cos, sin, mask, fused=None):
+    def forward_kv4(self, x, cache: KV4Cache, start, table, fused):
+        """Attention glue over a 4-bit cache: rotation and append in one launch, then attention; T tokens at consecutive positions
+        from ``start`` (int64 [1]) on."""
+        B, T = x.shape[0], x.shape[1]
+        H, Hkv, D = self.n_heads, self.n_kv_heads, self.head_dim
+        qkv = self.wqkv(x) if fused is None else self.wqkv.forward_normed(x, fused[0], fused[1])
+        q, k, v = qkv.view(B, T, H + 2 * Hkv, D).split([H, Hkv, Hkv], 2)
+        q = kv4_append(cache, k, v, start, q=q, table=table)
+        return self._project(kv4_attend(q, cache, start).reshape(B, T, H * D), x, fused)
+
+    def forward(self, x, cache: LayerCache, pos, cos, sin, mask, fused=None, table=None):
         """``fused`` = (norm weight, eps): the norm in front of wqkv runs in its front-end, x is wo's residual.  ``mask``: [1, 1,
-        T, L], or CAUSAL for one token per sequence, all at the same position (rotation, append and attention in one kernel)."""
+        T, L], or CAUSAL for one token per sequence, all at the same position (rotation, append and attention in one kernel).
+        ``table``: in place of cos and sin, for rotations of other layouts than adjacent pairs of the whole head."""
         B, T = x.shape[0], x.shape[1]
         H, Hkv, D = self.n_heads, self.n_kv_heads, self.head_dim
         qkv = self.wqkv(x) if fused is None else self.wqkv.forward_normed(x, fused[0], fused[1])
@@ -133,7 +151,7 @@ class Attention(nn.Module):
         q = qkv[..., : H * D].view(B, T, H, D)
         k = qkv[..., H * D: (H + Hkv) * D].view(B, T, Hkv, D)
         v = qkv[..., (H + Hkv) * D:].view(B, T, Hkv, D)
-        q, k = apply_rope(q, cos, sin), apply_rope(k, cos, sin)
+        q, k = rotate(q, k, table, pos) if table is not None else (apply_rope(q, cos, sin), apply_rope(k, cos, sin))
         ck, cv = cache                                  # [B, Hkv, L, D]
         ck.index_copy_(2, pos, k.transpose(1, 2))
         cv.index_copy_(2, pos, v.transpose(1, 2))
@@ -213,19 +231,23 @@ class TransformerBlock(nn.Module):
             self.attention_norm.weight.copy_(dic[prefix + ".attention_norm.weight"])
             self.ffn_norm.weight.copy_(dic[prefix + ".ffn_norm.weight"])
 
-    def forward(self, x, cache, pos, cos, sin, mask, fused: bool = False, flash=None):
+    def forward(self, x, cache, pos, cos, sin, mask, fused: bool = False, flash=None, table=None):
         if fused:
             eps = self.attention_norm.eps
             fused = (self.attention_norm.weight, eps)
-            if flash is not None:
+            if isinstance(cache, KV4Cache):
+                h = self.attention.forward_kv4(x, cache, pos[:1], table, fused)
+            elif flash is not None:
                 h = self.attention.forward_flash(x, cache, *flash, fused)
             else:
-                h = self.attention(x, cache, pos, cos, sin, mask, fused=fused)
+                h = self.attention(x, cache, pos, cos, sin, mask, fused=fused, table=table)
             return self.feed_forward.forward_fused(h, self.ffn_norm.weight, eps)
-        if flash is not None:
+        if isinstance(cache, KV4Cache):
+            h = x + self.attention.forward_kv4(self.attention_norm(x), cache, pos[:1], table, None)
+        elif flash is not None:
             h = x + self.attention.forward_flash(self.attention_norm(x), cache, *flash, None)
         else:
-            h = x + self.attention(self.attention_norm(x), cache, pos, cos, sin, mask)
+            h = x + self.attention(self.attention_norm(x), cache, pos, cos, sin, mask, table=table)
         return h + self.feed_forward(self.ffn_norm(h))
 
 
@@ -250,9 +272,16 @@ class Transformer(nn.Module):
         self.max_seq_len = max_seq_len
         self.tp = tp
         self._rope = None
+        self._table = None
         self.flash = False
+        if args.kv_bits not in (16, 4) or args.rope_layout not in LAYOUTS:
+            raise ValueError(f"kv_bits is 16 or 4 and rope_layout one of {LAYOUTS}: {args}")
+        if args.kv_bits == 4 and args.head_dim not in (64, 128):
+            raise ValueError(f"the 4-bit cache takes heads of 64 or 128 values, not {args.head_dim}")
+        # other layouts than adjacent pairs of the whole head, and the 4-bit cache, rotate by a RotaryTable
+        self._by_table = args.kv_bits == 4 or args.rope_layout != "interleaved" or args.rotary_dim not in (None, args.head_dim)
         want_flash = args.fused_glue if args.flash_attention is None else args.flash_attention
-        if want_flash and tp == 1:
+        if want_flash and tp == 1 and not self._by_table:
             try:
                 import flash_attn  # noqa: F401
                 self.flash = True
@@ -263,11 +292,18 @@ class Transformer(nn.Module):
 
     def make_cache(self, batch: int, device, dtype=torch.bfloat16) -> List[LayerCache]:
         a = self.args
+        if a.kv_bits == 4:
+            return [KV4Cache.empty(batch, a.n_kv_heads // self.tp, self.max_seq_len, a.head_dim, device) for _ in range(a.n_layers)]
         shape = (batch, a.n_kv_heads // self.tp, self.max_seq_len, a.head_dim)
         if self.flash:
             shape = (batch, self.max_seq_len, a.n_kv_heads, a.head_dim)
         return [(torch.zeros(shape, device=device, dtype=dtype), torch.zeros(shape, device=device, dtype=dtype))
                 for _ in range(a.n_layers)]
+
+    def _final_norm(self, h):
+        if self.args.fused_glue and h.is_cuda and h.dtype == torch.bfloat16 and h.shape[-1] % 16 == 0:
+            return rmsnorm(h, self.norm.weight, self.norm.eps)   # one launch, the fused front-ends' summation order
+        return self.norm(h)
 
     def head(self, h: torch.Tensor, greedy: bool = False):
         """Final norm + tied output head.  fp32 logits [B, T, vocab] (model.py:380-386 of the
@@ -275,10 +311,7 @@ class Transformer(nn.Module):
         Up to 8 rows run on the library's head kernel (one pass over the embedding, arg-max fused);
         more rows use the dense bf16 GEMM."""
         B, T = h.shape[0], h.shape[1]
-        if self.args.fused_glue and h.is_cuda and h.dtype == torch.bfloat16 and h.shape[-1] % 16 == 0:
-            h = rmsnorm(h, self.norm.weight, self.norm.eps)   # one launch, the fused front-ends' summation order
-        else:
-            h = self.norm(h)
+        h = self._final_norm(h)
         emb = self.tok_embeddings.weight
         if h.is_cuda and B * T <= 8 and emb.dtype == torch.bfloat16 and h.dtype == torch.bfloat16 and h.shape[-1] % 32 == 0:
             logits, toks = lm_head_argmax(h, emb, want_logits=not greedy, want_argmax=greedy)
@@ -287,25 +320,52 @@ class Transformer(nn.Module):
         logits = logits.float() if greedy else to_float(logits)
         return (None, logits.argmax(-1)) if greedy else logits
 
+    def _tables(self, device):
+        a = self.args
+        if self._rope is None or self._rope[0].device != device:
+            if self._by_table or a.rope_scaling is not None:
+                self._table = rotary_table(a.head_dim, self.max_seq_len, a.rope_theta, rotary_dim=a.rotary_dim, layout=a.rope_layout,
+                                           scaling=a.rope_scaling, device=device)
+                self._rope = (self._table.cos, self._table.sin)
+            else:
+                self._rope = rope_tables(a.head_dim, self.max_seq_len, a.rope_theta, device)
+            self._rope_lp = (self._rope[0].to(torch.bfloat16), self._rope[1].to(torch.bfloat16))
+
+    def score(self, tokens: torch.Tensor, cache: Optional[list] = None, top: int = 0) -> TokenLogprobs:
+        """Log probability of every token of [B, T] but the first, given those before it, with the entropies and, with ``top``, the most
+        probable alternatives there (scores.token_logprobs): [B, T - 1].  ``cache``: from make_cache, written from position 0 on; made here
+        if there is none."""
+        B, T = tokens.shape
+        if not 2 <= T <= self.max_seq_len:
+            raise ValueError(f"{T} tokens to score, 2 to {self.max_seq_len} wanted")
+        cache = self.make_cache(B, tokens.device) if cache is None else cache
+        h = self._hidden(tokens[:, :-1], cache, torch.arange(T - 1, device=tokens.device))
+        return token_logprobs(F.linear(self._final_norm(h), self.tok_embeddings.weight), tokens[:, 1:], top)
+
     def forward(self, tokens: torch.Tensor, cache: List[LayerCache], pos: torch.Tensor, greedy_last: bool = False):
         """tokens [B, T]; pos [T] (device int64) = positions written in the cache.
         Returns fp32 logits [B, T, vocab] (model.py:380-386 of the reference); with ``greedy_last``
         only the greedy token of every sequence's last position, int64 [B] (what the generation
         loop needs: generate.py:274, :283, :305 of the reference)."""
-        if self._rope is None or self._rope[0].device != tokens.device:
-            self._rope = rope_tables(self.args.head_dim, self.max_seq_len, self.args.rope_theta, tokens.device)
-            self._rope_lp = (self._rope[0].to(torch.bfloat16), self._rope[1].to(torch.bfloat16))
+        h = self._hidden(tokens, cache, pos)
+        if greedy_last:
+            return self.head(h[:, -1:], greedy=True)[1][:, 0]
+        return self.head(h)
+
+    def _hidden(self, tokens, cache, pos):
+        self._tables(tokens.device)
         B, T = tokens.shape
         h = self.tok_embeddings(tokens)
         fused = self.args.fused_glue and self.tp == 1
         flash, cos, sin, mask = None, None, None, None
-        if self.flash:   # the attention kernels apply RoPE from the tables and mask by position themselves
+        if self.args.kv_bits == 4:
+            pass             # rotation and visibility follow from the first position
+        elif self.flash:   # the attention kernels apply RoPE from the tables and mask by position themselves
             flash = (pos, self._rope_lp, tuple(t.index_select(0, pos) for t in self._rope_lp) if T == 1 else None)
         else:
-            cos, sin = self._rope[0][pos].expand(B, T, -1), self._rope[1][pos].expand(B, T, -1)
-            mask = CAUSAL if T == 1 else causal_mask(pos, self.max_seq_len)
+            if not self._by_table:
+                cos, sin = self._rope[0][pos].expand(B, T, -1), self._rope[1][pos].expand(B, T, -1)
+            mask = CAUSAL if T == 1 and not self._by_table else causal_mask(pos, self.max_seq_len)
         for layer, c in zip(self.layers, cache):
-            h = layer(h, c, pos, cos, sin, mask, fused, flash)
-        if greedy_last:
-            return self.head(h[:, -1:], greedy=True)[1][:, 0]
-        return self.head(h)
+            h = layer(h, c, pos, cos, sin, mask, fused, flash, self._table if self._by_table else None)
+        return h

@@ -282,6 +282,12 @@ def test_refusals(lib):
     for bad in (dict(max_len=0), dict(head_dim=96), dict(batch=0)):
         with pytest.raises(ValueError):
             KV4Cache.empty(**{**dict(batch=1, kv_heads=1, max_len=64, head_dim=64), **bad})
+    leaf = x.clone().requires_grad_()
+    for call in (lambda: kv4_append(cache, leaf, x, start), lambda: kv4_attend(leaf, cache, start)):
+        with pytest.raises(RuntimeError, match="gradient"):
+            call()
+    with torch.no_grad():
+        kv4_attend(leaf, cache, start)
     with pytest.raises(ValueError):
         KV4Cache(cache.k_codes[:, :, :60].contiguous(), *(t[:, :, :60].contiguous() for t in (cache.k_scales, cache.v_codes, cache.v_scales)))
     assert kv4_attend(x[:, :0], cache, start).shape == (2, 0, 2, 64) and kv4_append(cache, x[:, :0], x[:, :0], start) is None
