@@ -352,9 +352,11 @@ PyMethodDef layer_methods[] = {
 
 PyTypeObject layer_type = {PyVarObject_HEAD_INIT(nullptr, 0)};
 
-PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host_call", "Native call sites: the ternary linears and the packer.", -1, module_methods};
+PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host_call", "Native call sites: the ternary linears, the packer, the operators of rotary.py, kv4.py and scores.py.", -1, module_methods};
 
 }  // namespace
+
+extern PyMethodDef operator_methods[];   // host_operators.cpp
 
 PyMODINIT_FUNC PyInit__host_call() {
     static const char* const names[5] = {"weight_compressed_val", "weight_TileOffsets_global", "weight_TileOffsets_median", "weight_bitmap",
@@ -369,7 +371,7 @@ PyMODINIT_FUNC PyInit__host_call() {
     layer_type.tp_methods = layer_methods;
     if (PyType_Ready(&layer_type) < 0) return nullptr;
     PyObject* m = PyModule_Create(&module_def);
-    if (!m) return nullptr;
+    if (!m || PyModule_AddFunctions(m, operator_methods) < 0) return nullptr;
     Py_INCREF(&layer_type);
     PyModule_AddObject(m, "Layer", reinterpret_cast<PyObject*>(&layer_type));
     return m;

@@ -6,14 +6,12 @@ values.
 """
 from __future__ import annotations
 
-import ctypes
 from dataclasses import dataclass
 from typing import Optional
 
 import torch
 
-from .lib import load_library
-from .linear import _on, _stream
+from .lib import load_host_call
 from .rotary import RotaryTable
 
 GROUP = 32                # values that share a scale
@@ -62,39 +60,8 @@ class KV4Cache:
     def head_dim(self) -> int:
         return 2 * self.k_codes.shape[3]
 
-    def _ptrs(self):
-        return self.k_codes.data_ptr(), self.k_scales.data_ptr(), self.v_codes.data_ptr(), self.v_scales.data_ptr(), self.max_len
-
-
-def _check(cache: KV4Cache, name: str, x: Optional[torch.Tensor], heads: Optional[int]):
-    if not x.is_cuda:
-        raise RuntimeError(f"{name} needs CUDA tensors: the B200 library has no CPU path")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError(f"{name} requires a gradient: the 4-bit cache has none")
-    if (x.dim() != 4 or x.dtype != torch.bfloat16 or x.device != cache.k_codes.device or x.shape[0] != cache.batch or x.shape[3] != cache.head_dim
-            or x.shape[2] == 0 or (heads is not None and x.shape[2] != heads)):
-        raise ValueError(f"{name}: bf16 [{cache.batch}, T, {heads or 'heads'}, {cache.head_dim}] on {cache.k_codes.device} wanted, not {x.dtype} {list(x.shape)} on {x.device}")
-
-
-def _check_places(cache: KV4Cache, start: torch.Tensor, counts: Optional[torch.Tensor]):
-    for name, t, sizes in (("start", start, (1, cache.batch)), ("counts", counts, (cache.batch,))):
-        if t is not None and (t.dtype != torch.int64 or t.dim() != 1 or t.shape[0] not in sizes or not t.is_contiguous() or t.device != cache.k_codes.device):
-            raise ValueError(f"{name} is contiguous int64 [{cache.batch}] on {cache.k_codes.device}, not {t.dtype} {list(t.shape)}")
-
-
-def _aligned(x: torch.Tensor, to: int):
-    """x with contiguous heads whose rows start on multiples of ``to`` bytes."""
-    ok = x.stride(3) == 1 and x.data_ptr() % to == 0 and all(s % (to // 2) == 0 for s in x.stride()[:3])
-    return x if ok else x.contiguous()
-
-
-def _strides(t: torch.Tensor):
-    return (ctypes.c_longlong * 3)(*t.stride()[:3])
-
-
-def _raise(status: int, name: str):
-    if status:
-        raise RuntimeError(f"{name}: status {status}")
+    def _tensors(self):
+        return self.k_codes, self.k_scales, self.v_codes, self.v_scales
 
 
 def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor, counts: Optional[torch.Tensor] = None,
@@ -103,50 +70,14 @@ def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, start: torch.T
     cache, ``start`` int64 [B] or [1] on the device; of sequence b only the first counts[b], rows behind those stay as they were.  With ``table``
     keys - and queries bf16 [B, T, H, D], whose rotated form is returned - are turned by their positions first, in the same
     launch.  A sequence that does not fit is not written, and the library's status is 1."""
-    _check(cache, "k", k, cache.kv_heads)
-    _check(cache, "v", v, cache.kv_heads)
-    if v.shape != k.shape:
-        raise ValueError(f"k and v have one shape, not {list(k.shape)} and {list(v.shape)}")
-    _check_places(cache, start, counts)
-    if table is not None and (table.rotary_dim > cache.head_dim or table.cos.device != k.device):
-        raise ValueError(f"the table rotates {table.rotary_dim} values on {table.cos.device}, a head has {cache.head_dim} on {k.device}")
-    B, T = k.shape[:2]
-    out = None
-    if q is not None:
-        if table is None:
-            raise ValueError("queries are only passed to be rotated: table is missing")
-        _check(cache, "q", q, None)
-        if q.shape[1] != T:
-            raise ValueError(f"{q.shape[1]} queries beside {T} keys")
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        q = _aligned(q, 8)
-    if T == 0:
-        return out
-    k, v = _aligned(k, 8), _aligned(v, 8)
-    with _on(k):
-        _raise(load_library().ternaspmm_kv4_append(
-            *cache._ptrs(), k.data_ptr(), _strides(k), v.data_ptr(), _strides(v), None if q is None else q.data_ptr(), None if q is None else _strides(q),
-            None if q is None else out.data_ptr(), None if table is None else table.cos.data_ptr(), None if table is None else table.sin.data_ptr(),
-            0 if table is None else table.max_len, 0 if table is None else table.rotary_dim, table is not None and table.layout == "half",
-            start.data_ptr(), start.shape[0] > 1, None if counts is None else counts.data_ptr(), B, T, 0 if q is None else q.shape[2],
-            cache.kv_heads, cache.head_dim, _stream()), "kv4_append")
-    return out
+    cos, sin, half = (None, None, False) if table is None else (table.cos, table.sin, table.layout == "half")
+    return load_host_call().kv4_append(*cache._tensors(), k, v, start, counts, q, cos, sin, half)
 
 
 def kv4_read(cache: KV4Cache, start: torch.Tensor, tokens: int, counts: Optional[torch.Tensor] = None):
     """The keys and values that rows start[b] .. start[b] + tokens - 1 stand for, bf16 [B, tokens, Hkv, D] each; zeros behind a sequence's
     counts[b]."""
-    _check_places(cache, start, counts)
-    if tokens < 0:
-        raise ValueError(f"{tokens} tokens")
-    if not cache.k_codes.is_cuda:
-        raise RuntimeError("kv4_read needs CUDA tensors: the B200 library has no CPU path")
-    k, v = (torch.empty((cache.batch, tokens, cache.kv_heads, cache.head_dim), dtype=torch.bfloat16, device=cache.k_codes.device) for _ in range(2))
-    if tokens:
-        with _on(k):
-            _raise(load_library().ternaspmm_kv4_read(*cache._ptrs(), start.data_ptr(), start.shape[0] > 1, None if counts is None else counts.data_ptr(),
-                                                     k.data_ptr(), v.data_ptr(), cache.batch, tokens, cache.kv_heads, cache.head_dim, _stream()), "kv4_read")
-    return k, v
+    return load_host_call().kv4_read(*cache._tensors(), start, tokens, counts)
 
 
 def kv4_attend(q: torch.Tensor, cache: KV4Cache, start: torch.Tensor, counts: Optional[torch.Tensor] = None, window: int = 0,
@@ -155,23 +86,4 @@ def kv4_attend(q: torch.Tensor, cache: KV4Cache, start: torch.Tensor, counts: Op
     and ``counts`` as in ``kv4_append``.  The query of token t sees the keys up to position start[b] + t, below start[b] + counts[b],
     and with ``window`` only the last ``window`` of them; a query that sees none gives zeros.  ``scale`` of the scores: 1 / sqrt(D).  bf16
     [B, T, H, D].  A sequence outside of the cache gives NaN and status 1 of the library."""
-    _check(cache, "q", q, None)
-    _check_places(cache, start, counts)
-    B, T, H, D = q.shape
-    if H % cache.kv_heads:
-        raise ValueError(f"{H} query heads over {cache.kv_heads} key heads")
-    scale = D ** -0.5 if scale is None else float(scale)
-    if window < 0 or window >= 1 << 31 or not 0 < scale <= 1e6:
-        raise ValueError(f"window {window}, scale {scale}")
-    out = torch.empty((B, T, H, D), dtype=torch.bfloat16, device=q.device)
-    if T == 0:
-        return out
-    q = _aligned(q, 16)
-    lib = load_library()
-    with _on(q):
-        need = lib.ternaspmm_kv4_attend_workspace(B, T, H, cache.kv_heads, D, cache.max_len)
-        work = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
-        _raise(lib.ternaspmm_kv4_attend(q.data_ptr(), _strides(q), *cache._ptrs(), start.data_ptr(), start.shape[0] > 1,
-                                        None if counts is None else counts.data_ptr(), window, scale, out.data_ptr(), B, T, H, cache.kv_heads, D,
-                                        None if work is None else work.data_ptr(), max(need, 0), _stream()), "kv4_attend")
-    return out
+    return load_host_call().kv4_attend(q, *cache._tensors(), start, counts, window, scale)

@@ -2,22 +2,19 @@
 
 ``linear.rope`` and the attention kernels rotate adjacent pairs of a whole head of 128 by the reference's unscaled angles
 (model.py:205-243 of Gu-J/TernaInfer).  Here are the other forms that checkpoints are trained with: pairs of the two halves, a
-part of the head, and angles scaled for contexts longer than the trained ones.  Kernel: csrc/rotary.cuh.
+part of the head, and angles scaled for contexts longer than the trained ones.  Kernel: csrc/rotary.cuh; call site: csrc/host_operators.cpp.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 from dataclasses import dataclass
 from typing import Optional
 
 import torch
 
-from .lib import load_library
-from .linear import _on, _stream
+from .lib import load_host_call
 
 LAYOUTS = ("interleaved", "half")
-_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
 @dataclass(frozen=True)
@@ -101,71 +98,8 @@ def rotary_table(head_dim: int, max_len: int, theta: float = 10000.0, *, rotary_
     return RotaryTable((angle.cos() * factor).float(), (angle.sin() * factor).float(), layout)
 
 
-def _strides(t: torch.Tensor):
-    return (ctypes.c_longlong * 3)(*t.stride()[:3])
-
-
-def _takes(x: torch.Tensor, layout: str):
-    """x as the kernel reads it: contiguous heads, whole pairs on their boundaries in the interleaved layout."""
-    if x.stride(3) != 1 or (layout == "interleaved" and (any(s % 2 for s in x.stride()[:3]) or x.data_ptr() % (2 * x.element_size()))):
-        return x.contiguous()
-    return x
-
-
-def _launch(q, k, table, positions, inverse):
-    B, T, H, D = q.shape
-    q, k = _takes(q, table.layout), None if k is None else _takes(k, table.layout)
-    out = torch.empty((B, T, H, D), dtype=q.dtype, device=q.device)
-    k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    if q.numel() == 0:
-        return out, k_out
-    shared = positions.dim() == 1
-    with _on(q):
-        status = load_library().ternaspmm_rotate(
-            q.data_ptr(), _strides(q), H, out.data_ptr(), None if k is None else k.data_ptr(), None if k is None else _strides(k),
-            0 if k is None else k.shape[2], None if k is None else k_out.data_ptr(), _TYPES[q.dtype], table.cos.data_ptr(), table.sin.data_ptr(),
-            table.max_len, table.rotary_dim, table.layout == "half", inverse, positions.data_ptr(), 0 if shared else positions.stride(0),
-            positions.stride(-1), B, T, D, _stream())
-    if status:
-        raise RuntimeError(f"ternaspmm_rotate: status {status}")
-    return out, k_out
-
-
-class _Rotate(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, cos, sin, layout, positions):
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(cos, sin, positions)
-        ctx.layout = layout
-        return _launch(q, k, RotaryTable(cos, sin, layout), positions, False)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gq, gk):
-        cos, sin, positions = ctx.saved_tensors
-        table = RotaryTable(cos, sin, ctx.layout)
-        gq, gk = (g if need else None for g, need in zip((gq, gk), ctx.needs_input_grad))
-        if gq is not None:
-            gq, gk = _launch(gq, gk, table, positions, True)
-        elif gk is not None:
-            gk = _launch(gk, None, table, positions, True)[0]
-        return gq, gk, None, None, None, None
-
-
 def rotate(q: torch.Tensor, k: Optional[torch.Tensor], table: RotaryTable, positions: torch.Tensor):
     """Queries [B, T, H, D] and keys [B, T, Hkv, D] (or None) turned by the angles of their positions, in one launch: (q, k) of the same type
     (bf16, fp16 or fp32), products in fp32, rounded once.  ``positions``: int64 [T] or [B, T] on the device.  Strided views are taken as
     they are.  Differentiable in q and k.  A position outside of the table gives NaN in its token and status 1 of the library."""
-    if not q.is_cuda:
-        raise RuntimeError("rotate needs CUDA tensors: the B200 library has no CPU path")
-    if q.dim() != 4 or q.dtype not in _TYPES or q.shape[3] % 2:
-        raise ValueError(f"q is bf16, fp16 or fp32 [B, T, H, D] with an even D, not {q.dtype} {list(q.shape)}")
-    if k is not None and (k.dim() != 4 or k.dtype != q.dtype or k.device != q.device or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3]):
-        raise ValueError(f"k is {q.dtype} [B, T, Hkv, D] beside q, not {k.dtype} {list(k.shape)}")
-    if positions.dtype != torch.int64 or positions.device != q.device or list(positions.shape) not in ([q.shape[1]], list(q.shape[:2])):
-        raise ValueError(f"positions are int64 [T] or [B, T] on {q.device}, not {positions.dtype} {list(positions.shape)}")
-    if table.rotary_dim > q.shape[3] or table.cos.device != q.device:
-        raise ValueError(f"the table rotates {table.rotary_dim} values on {table.cos.device}, a head has {q.shape[3]} on {q.device}")
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _Rotate.apply(q, k, table.cos, table.sin, table.layout, positions)
-    return _launch(q, k, table, positions, False)
+    return load_host_call().rotate(q, k, table.cos, table.sin, table.layout == "half", positions)

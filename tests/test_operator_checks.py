@@ -23,6 +23,8 @@ def test_cpu_tensors_are_refused():
                  lambda: kv4_attend(x, cache, pos[:1]), lambda: token_logprobs(torch.zeros((2, 5)), pos)):
         with pytest.raises(RuntimeError, match="no CPU path"):
             call()
+    with pytest.raises(ValueError, match="-12 tokens"):      # (a message with a number: the extension and torch share one libstdc++)
+        kv4_read(cache, pos[:1], -12)
 
 
 def test_cache_shapes():
