@@ -47,7 +47,8 @@ def attention(q, k, v, start, counts, window, scale):
     s = s.masked_fill(~sees[:, None], -math.inf)
     p = torch.softmax(s, -1).nan_to_num(0.0)
     out = torch.einsum("bhtl,blhd->bthd", p, vv)
-    # The result is rounded to bf16: 2^-8.  Probabilities times scales are rounded to fp16: 2^-11 of each term; below 2^-14 of the largest
+    # The result is rounded to bf16: 2^-8.  Probabilities are rounded to fp16, and so are their products with the scales: 2^-11 of each
+    # term twice, 2^-10 + 2^-22 together, and 2^-13 for exponentials and sums; below 2^-14 of the largest
     # scale by up to 2^-25 of it, times |code - 8| <= 8.  Scores: fp32 sums of exact products, 128 of them, then a few roundings:
     # 2^-16 of sum |q||k| each at most, as an exponent.  The two accumulators of a value run over codes up to 15 and over the offset of 8, so they
     # are up to 15 / 8 of the largest value where the result may be next to nothing: each MMA, one for each of at most n / 16 + 1 groups
@@ -56,7 +57,7 @@ def attention(q, k, v, start, counts, window, scale):
     top = vv.abs().amax((1, 3))[:, None, :, None]
     n = float(counts.max() + start.max()) + 1
     q_size = (q.double().abs().amax(-1) * q.shape[-1]).permute(0, 2, 1) * kk.abs().amax((1, 3))[:, :, None] * scale
-    lost = size * (2.0 ** -11 + 2.0 ** -12) + top * (n * 2.0 ** -24 * 2 + (n / 16 + 1) * 2.0 ** -21) + \
+    lost = size * (2.0 ** -10 + 2.0 ** -13) + top * (n * 2.0 ** -24 * 2 + (n / 16 + 1) * 2.0 ** -21) + \
         (q_size * 2.0 ** -20).permute(0, 2, 1)[..., None] * size
     # What is rounded to bf16 is the result with those errors: |r(out + e) - out| <= |e| + 2^-8 |out + e| <= lost + 2^-8 (|out| + lost)
     return out, lost + (out.abs() + lost) * 2.0 ** -8
