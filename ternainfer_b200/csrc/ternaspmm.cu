@@ -1286,23 +1286,22 @@ extern "C" int ternaspmm_kv4_read(void* k_codes, void* k_scales, void* v_codes, 
     return t_host_status;
 }
 
-// How an attention call is cut: tiles of 8 query rows per CTA, CTAs for the rows of a key / value head, splits over the keys, and
-// whether the splits of an item are a cluster.
+// How an attention call is cut: tiles of 8 query rows per CTA, CTAs for the rows of a key / value head, and CTAs of a cluster for
+// each or, with `stream`, that many CTAs for everything.
 struct Kv4Plan {
-    int tiles, row_tiles, splits;
-    bool cluster;
+    int tiles, row_tiles, cluster, stream;
 };
 static Kv4Plan kv4_plan(int batch, int tokens, int heads, int kv_heads, int max_len) {
     const long long rows_all = (long long)tokens * (heads / kv_heads);
-    Kv4Plan pl;
-    pl.tiles = rows_all <= 8 ? 1 : 2;
+    Kv4Plan pl = {rows_all <= 8 ? 1 : 2, 1, 1, 0};
     pl.row_tiles = (int)((rows_all + 8 * pl.tiles - 1) / (8 * pl.tiles));
-    const long long items = (long long)batch * kv_heads * pl.row_tiles, slots = (pl.tiles == 1 ? 4ll : 2ll) * device_sm_count();
-    const long long most = (max_len / 32 + kKv4Warps - 1) / kKv4Warps;
-    pl.splits = 1;
-    while (pl.splits < 8 && pl.splits < most && items * pl.splits < 4 * slots) pl.splits *= 2;
-    pl.cluster = pl.splits > 1;
-    if (items * 16 <= slots && most > 16) pl.splits = (int)std::min(std::min(slots / items, most), 1024ll), pl.cluster = false;
+    const int slots = (pl.tiles == 1 ? 4 : 2) * device_sm_count();
+    const long long items = (long long)batch * kv_heads * pl.row_tiles, blocks = max_len / 32;
+    if (pl.row_tiles == 1 && items * blocks >= 4ll * kKv4Warps * slots) {
+        pl.stream = slots;
+        return pl;
+    }
+    while (pl.cluster < 8 && pl.cluster * kKv4Warps < blocks && items * pl.cluster < 2 * slots) pl.cluster *= 2;
     return pl;
 }
 static bool kv4_attend_shape(int batch, int tokens, int heads, int kv_heads, int head_dim, int max_len) {
@@ -1312,43 +1311,50 @@ static bool kv4_attend_shape(int batch, int tokens, int heads, int kv_heads, int
 extern "C" long long ternaspmm_kv4_attend_workspace(int batch, int tokens, int heads, int kv_heads, int head_dim, int max_len) {
     if (!kv4_attend_shape(batch, tokens, heads, kv_heads, head_dim, max_len)) return -1;
     const Kv4Plan pl = kv4_plan(batch, tokens, heads, kv_heads, max_len);
-    return pl.splits == 1 || pl.cluster ? 0 : (long long)batch * kv_heads * pl.row_tiles * pl.splits * 8 * pl.tiles * (head_dim + 2) * 4;
+    return (long long)pl.stream * 2 * 8 * pl.tiles * (head_dim + 2) * 4;
 }
 
 template <int D, int NT>
-static cudaError_t launch_kv4_attend(const Kv4AttnParams& p, int batch, bool cluster, cudaStream_t stream) {
-    constexpr int smem = kKv4Warps * Kv4Stage<D>::ring + kKv4BarBytes;
+static cudaError_t launch_kv4_attend(const Kv4AttnParams& p, int stream_ctas, cudaStream_t stream) {
+    constexpr int smem = kKv4Warps * Kv4Stage<D>::ring + Kv4Stage<D>::frags(NT);
     static_assert(Kv4Stage<D>::ring >= 8 * NT * D * 4, "the partial results of the warps lie where their rings were");
+    static_assert(Kv4Stage<D>::frags(NT) >= (kKv4Warps + 1) * 8 * NT * 8, "the statistics of the results lie where the query's fragments were");
     static bool done[64] = {false};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64) dev = 0;
     if (!done[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(kv4_attn_kernel<D, NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4_attn_kernel<D, NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        cudaError_t e = cudaFuncSetAttribute(kv4_attn_kernel<D, NT, KV4_CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4_attn_kernel<D, NT, KV4_STREAM>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return e;
         done[dev] = true;
     }
     cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = p.splits;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((long long)p.splits * p.row_tiles * p.c.kv_heads), batch, 1);
     cfg.blockDim = dim3(kKv4Warps * 32, 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cfg.attrs = attr;
-    cfg.numAttrs = cluster ? 1 : 0;
-    cudaError_t e = cluster ? cudaLaunchKernelEx(&cfg, kv4_attn_kernel<D, NT, true>, p) : cudaLaunchKernelEx(&cfg, kv4_attn_kernel<D, NT, false>, p);
-    if (e != cudaSuccess || p.splits == 1 || cluster) return e;
+    if (!stream_ctas) {
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = p.cluster;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.gridDim = dim3((unsigned)((long long)p.cluster * p.row_tiles * p.c.kv_heads), p.batch, 1);
+        cfg.numAttrs = p.cluster > 1 ? 1 : 0;
+        return cudaLaunchKernelEx(&cfg, kv4_attn_kernel<D, NT, KV4_CLUSTER>, p);
+    }
+    cfg.gridDim = dim3(stream_ctas, 1, 1);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kv4_attn_kernel<D, NT, KV4_STREAM>, p);
+    if (e != cudaSuccess) return e;
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3((unsigned)(8 * NT * p.row_tiles * p.c.kv_heads), batch, 1);
-    cfg.blockDim = dim3(D, 1, 1);
+    // a CTA per row where all fit beside each other (the parts of a row are many then: one sequence, 118 of them, 46.4 -> 38.2 us), else per item
+    const int rows = p.tokens * (p.heads / p.c.kv_heads), here = (long long)p.batch * p.c.kv_heads * rows <= device_sm_count() ? 1 : rows;
+    cfg.gridDim = dim3((unsigned)(p.c.kv_heads * (rows / here)), p.batch, 1);
+    cfg.blockDim = dim3(kKv4JoinWarps * 32, 1, 1);
     cfg.dynamicSmemBytes = 0;
     cfg.numAttrs = tuning().pdl ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kv4_attn_join_kernel<D, NT>, p);
+    return cudaLaunchKernelEx(&cfg, kv4_attn_join_kernel<D, NT>, p, stream_ctas, here);
 }
 
 extern "C" int ternaspmm_kv4_attend(const __nv_bfloat16* q, const long long* q_strides, void* k_codes, void* k_scales, void* v_codes, void* v_scales,
@@ -1366,11 +1372,11 @@ extern "C" int ternaspmm_kv4_attend(const __nv_bfloat16* q, const long long* q_s
     if (!p.status) return t_host_status = ST_LAUNCH;
     const Kv4Plan pl = kv4_plan(batch, tokens, heads, kv_heads, max_len);
     p.start = start, p.counts = counts, p.start_stride = start_stride ? 1 : 0, p.out = out, p.tokens = tokens, p.heads = heads, p.window = window;
-    p.splits = pl.splits, p.row_tiles = pl.row_tiles, p.row_bytes = head_dim / 2, p.scale_log2 = scale * 1.4426950408889634f;
+    p.batch = batch, p.cluster = pl.cluster, p.row_tiles = pl.row_tiles, p.row_bytes = head_dim / 2, p.scale_log2 = scale * 1.4426950408889634f;
     p.part_o = static_cast<float*>(workspace);
-    p.part_ml = reinterpret_cast<float2*>(p.part_o + (size_t)batch * kv_heads * pl.row_tiles * pl.splits * 8 * pl.tiles * head_dim);
-    const cudaError_t e = head_dim == 128 ? (pl.tiles == 1 ? launch_kv4_attend<128, 1>(p, batch, pl.cluster, stream) : launch_kv4_attend<128, 2>(p, batch, pl.cluster, stream))
-                                          : (pl.tiles == 1 ? launch_kv4_attend<64, 1>(p, batch, pl.cluster, stream) : launch_kv4_attend<64, 2>(p, batch, pl.cluster, stream));
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + (size_t)pl.stream * 2 * 8 * pl.tiles * head_dim);
+    const cudaError_t e = head_dim == 128 ? (pl.tiles == 1 ? launch_kv4_attend<128, 1>(p, pl.stream, stream) : launch_kv4_attend<128, 2>(p, pl.stream, stream))
+                                          : (pl.tiles == 1 ? launch_kv4_attend<64, 1>(p, pl.stream, stream) : launch_kv4_attend<64, 2>(p, pl.stream, stream));
     if (e != cudaSuccess) t_host_status = ST_LAUNCH;
     checkLastCudaError(__LINE__);
     return t_host_status;

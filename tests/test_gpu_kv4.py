@@ -165,6 +165,35 @@ def test_attend_window_and_ragged(lib, window, T):
     check(q, cache, k, v, start, counts=torch.tensor([T, T // 2, 0, T, 1], device="cuda"), window=window)
 
 
+@pytest.mark.parametrize("D,H,K,T", [(128, 8, 2, 1), (64, 5, 5, 1), (128, 12, 1, 1), (128, 4, 2, 3), (64, 3, 1, 5)])
+def test_attend_sequences_of_all_lengths(lib, D, H, K, T):
+    """Caches large enough for the work to be cut across sequences: empty ones, one key, whole tiles and ragged ones beside each other; less work
+    than there are CTAs; windows; some outside of the cache."""
+    B, L = 40, 8192 // K
+    cache, k, v = filled(B, K, L, D, T)
+    q = torch.randn((B, T, H, D), generator=gen(H), device="cuda").to(torch.bfloat16)
+    g = gen(12)
+    full = torch.full((B,), T, device="cuda")
+    ragged = torch.randint(0, L - T + 1, (B,), generator=g, device="cuda")
+    ragged[[0, 7, 8, 39]], ragged[3], ragged[4], ragged[20] = 0, 31, 32, L - T
+    counts = full.clone()
+    counts[[1, 7, 8, 30]] = 0
+    empty = torch.zeros_like(ragged)
+    one = empty.clone()
+    one[11] = min(2000, L - 9)                # (within every one of these caches)
+    for start, c, window in ((ragged, None, 0), (ragged, counts, 0), (ragged, None, 100), (empty, None, 0), (empty, empty, 0), (one, counts, 0), (empty + L - T, None, 0)):
+        check(q, cache, k, v, start, counts=c, window=window)
+    assert lib.ternaspmm_last_status() == 0
+    bad = ragged.clone()
+    bad[[5, 39]] = torch.tensor([cache.max_len, -1], device="cuda")      # (the capacity: L rounded up)
+    out = kv4_attend(q, cache, bad)
+    assert out.isnan().flatten(1).all(1).nonzero().flatten().tolist() == [5, 39] and lib.ternaspmm_last_status() == 1
+    good = torch.ones(B, dtype=torch.bool, device="cuda")
+    good[[5, 39]] = False
+    ref, tol = attention(q[good], k[good], v[good], bad[good], full[good], 0, D ** -0.5)
+    assert ((out[good].double() - ref).abs() <= tol).all()
+
+
 def test_attend_long_cache(lib):
     """One sequence, more keys than any split takes in one go; the last keys alone decide, then the first."""
     B, H, K, D, L = 1, 8, 2, 128, 70000
