@@ -376,8 +376,9 @@ long long ternaspmm_kv4_attend_workspace(int batch, int tokens, int heads, int k
  * first among equal logits (NaN before all).  _grad: grad [rows][vocab] contiguous, of the logits' type, from the gradients of log probability
  * and entropy (either may be null). */
 int ternaspmm_token_logprobs(const void* logits, long long ld, int type, const long long* targets, int rows, int vocab, int top,
-                             float* logprob, float* entropy, float* lse, float* top_logprob, long long* top_token,
-                             ternaspmm_stream_t stream);
+                             float* logprob, float* entropy, float* lse, float* top_logprob, long long* top_token, void* workspace,
+                             long long workspace_bytes, ternaspmm_stream_t stream);
+long long ternaspmm_token_logprobs_workspace(int rows, int vocab, int type, int top);
 int ternaspmm_token_logprobs_grad(const void* logits, long long ld, int type, const long long* targets, int rows, int vocab,
                                   const float* lse, const float* entropy, const float* g_logprob, const float* g_entropy, void* grad,
                                   ternaspmm_stream_t stream);

@@ -1383,19 +1383,68 @@ extern "C" int ternaspmm_kv4_attend(const __nv_bfloat16* q, const long long* q_s
 }
 
 // ---- log probabilities of given tokens (logprobs.cuh) -------------------------------------------------
+static int logprob_parts(int vocab, int type) {
+    const int part = kLpPartBytes / (type == 2 ? 4 : 2);
+    return (vocab + part - 1) / part;
+}
+static bool logprob_shape(int rows, int vocab, int type, int top) {
+    return rows >= 1 && vocab >= 1 && vocab <= kLpMaxVocab && type >= 0 && type <= 2 && top >= 0 && top <= kLpMaxTop && top <= vocab;
+}
+
+extern "C" long long ternaspmm_token_logprobs_workspace(int rows, int vocab, int type, int top) {
+    if (!logprob_shape(rows, vocab, type, top)) return -1;
+    return (long long)rows * logprob_parts(vocab, type) * (kLpWarps * 16 + 8 * top);
+}
+
+template <typename T>
+static cudaError_t launch_logprobs(const LogprobParams& p, cudaStream_t stream) {
+    static bool done[64] = {false};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) dev = 0;
+    const int join_smem = p.lists * (8 * p.top + 4);
+    static_assert((kLpMaxVocab * 4 / kLpPartBytes + 1) * (8 * kLpMaxTop + 4) <= 48 * 1024, "the lists of a row's parts fit into shared memory");
+    if (!done[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(logprob_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kLpPartBytes);
+        if (e != cudaSuccess) return e;
+        done[dev] = true;
+    }
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)std::min((long long)p.rows * p.lists, (long long)kLpCtasPerSm * device_sm_count()), 1, 1);
+    cfg.blockDim = dim3(kLpThreads, 1, 1);
+    cfg.dynamicSmemBytes = 2 * kLpPartBytes;
+    cfg.stream = stream;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, logprob_kernel<T>, p);
+    if (e != cudaSuccess) return e;
+    cfg.gridDim = dim3((unsigned)p.rows, 1, 1);
+    cfg.blockDim = dim3(32, 1, 1);
+    cfg.dynamicSmemBytes = join_smem;
+    cfg.attrs = attr;
+    cfg.numAttrs = tuning().pdl ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, logprob_join_kernel<T>, p);
+}
+
 extern "C" int ternaspmm_token_logprobs(const void* logits, long long ld, int type, const long long* targets, int rows, int vocab, int top,
-                                        float* logprob, float* entropy, float* lse, float* top_logprob, long long* top_token, cudaStream_t stream) {
+                                        float* logprob, float* entropy, float* lse, float* top_logprob, long long* top_token, void* workspace,
+                                        long long workspace_bytes, cudaStream_t stream) {
     t_host_status = ST_OK;
-    if (rows < 1 || vocab < 1 || ld < vocab || type < 0 || type > 2 || top < 0 || top > kLpMaxTop || top > vocab) return t_host_status = ST_BAD_SHAPE;
-    LogprobParams p = {logits, ld, targets, logprob, entropy, lse, top_logprob, top_token, vocab, top, status_device_ptr()};
-    if (!logits || !targets || !logprob || !entropy || !lse || (top && (!top_logprob || !top_token)) || reinterpret_cast<uintptr_t>(logits) % (type == 2 ? 4 : 2))
+    if (!logprob_shape(rows, vocab, type, top) || ld < vocab || workspace_bytes < ternaspmm_token_logprobs_workspace(rows, vocab, type, top))
+        return t_host_status = ST_BAD_SHAPE;
+    LogprobParams p = {logits, ld, targets, logprob, entropy, lse, top_logprob, top_token, static_cast<float*>(workspace), nullptr, rows, vocab, top,
+                       logprob_parts(vocab, type), 1, 1, status_device_ptr()};
+    // up to eight parts of a row in turn, as long as every CTA has at least two such runs (one where the alternatives are not asked for: nothing
+    // is carried from part to part then)
+    if (top) p.run = (int)std::max(1ll, std::min(8ll, (long long)rows * p.parts / (2ll * kLpCtasPerSm * device_sm_count())));
+    p.lists = (p.parts + p.run - 1) / p.run;
+    p.keys = reinterpret_cast<unsigned long long*>(p.sums + (size_t)rows * p.parts * kLpWarps * 4);
+    if (!logits || !targets || !logprob || !entropy || !lse || !workspace || (top && (!top_logprob || !top_token)) ||
+        reinterpret_cast<uintptr_t>(logits) % (type == 2 ? 4 : 2) || (reinterpret_cast<uintptr_t>(workspace) & 15))
         return t_host_status = ST_BAD_POINTER;
     if (!p.status) return t_host_status = ST_LAUNCH;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)rows, 1, 1);
-    cfg.blockDim = dim3(kLpThreads, 1, 1);
-    cfg.stream = stream;
-    if (cudaLaunchKernelEx(&cfg, type == 0 ? logprob_kernel<__nv_bfloat16> : type == 1 ? logprob_kernel<__half> : logprob_kernel<float>, p) != cudaSuccess)
+    if ((type == 0 ? launch_logprobs<__nv_bfloat16>(p, stream) : type == 1 ? launch_logprobs<__half>(p, stream) : launch_logprobs<float>(p, stream)) != cudaSuccess)
         t_host_status = ST_LAUNCH;
     checkLastCudaError(__LINE__);
     return t_host_status;

@@ -144,11 +144,13 @@ def load_library() -> ctypes.CDLL:
                        ("ternaspmm_kv4_append", [_P] * 4 + [_I] + [_P] * 9 + [_I] * 3 + [_P, _I, _P] + [_I] * 5 + [_P]),
                        ("ternaspmm_kv4_read", [_P] * 4 + [_I, _P, _I, _P, _P, _P] + [_I] * 4 + [_P]),
                        ("ternaspmm_kv4_attend", [_P] * 6 + [_I, _P, _I, _P, _I, ctypes.c_float, _P] + [_I] * 5 + [_P, _L, _P]),
-                       ("ternaspmm_token_logprobs", [_P, _L, _I, _P, _I, _I, _I] + [_P] * 6),
+                       ("ternaspmm_token_logprobs", [_P, _L, _I, _P, _I, _I, _I] + [_P] * 6 + [_L, _P]),
                        ("ternaspmm_token_logprobs_grad", [_P, _L, _I, _P, _I, _I] + [_P] * 6)):
         fn = getattr(lib, name)
         fn.argtypes = args
         fn.restype = _I
+    lib.ternaspmm_token_logprobs_workspace.argtypes = [_I] * 4
+    lib.ternaspmm_token_logprobs_workspace.restype = _L
     lib.ternaspmm_kv4_attend_workspace.argtypes = [_I] * 6
     lib.ternaspmm_kv4_attend_workspace.restype = _L
     lib.ternaspmm_pack_i8.argtypes = [_P, _I, _I, _P, _P, _P, _P]
@@ -187,6 +189,6 @@ EXPORTED_SYMBOLS = (
     "ternaspmm_scale_quant_sumsq", "ternaspmm_partial_f32", "ternaspmm_tp_finish", "ternaspmm_tp_allreduce_finish", "ternaspmm_rmsnorm_quant", "ternaspmm_relu2_gate_rmsnorm_quant", "ternaspmm_rmsnorm", "ternaspmm_pack_i8",
     "ternaspmm_w2_relayout", "ternaspmm_rope", "ternaspmm_relu2_gate", "ternaspmm_bf16_to_f32", "ternaspmm_attn_decode", "ternaspmm_attn_decode_by_head", "ternaspmm_attn_prefill", "ternaspmm_pack_gpu_layout", "ternaspmm_pack_gpu_signs", "ternaspmm_w2_bytes", "ternaspmm_w2_pays", "ternaspmm_w2_fused_rows", "ternaspmm_w2_linear",
     "ternaspmm_rotate", "ternaspmm_kv4_append", "ternaspmm_kv4_read", "ternaspmm_kv4_attend", "ternaspmm_kv4_attend_workspace",
-    "ternaspmm_token_logprobs", "ternaspmm_token_logprobs_grad",
+    "ternaspmm_token_logprobs", "ternaspmm_token_logprobs_workspace", "ternaspmm_token_logprobs_grad",
     "ternaspmm_unpack_i8", "ternaspmm_transcode_reference_layout",
 )
