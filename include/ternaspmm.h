@@ -372,7 +372,7 @@ int ternaspmm_kv4_attend(const ternaspmm_bf16* q, const long long* q_strides, vo
 long long ternaspmm_kv4_attend_workspace(int batch, int tokens, int heads, int kv_heads, int head_dim, int max_len);
 
 /* Per row of logits [rows][vocab] (type as above, `ld` elements between rows): log probability of targets[row] (int64; negative: no
- * token, 0), entropy, log of the sum of exponentials, and the `top` <= 32 most probable tokens with their log probabilities, the lowest id
+ * token, 0), entropy, log of the sum of exponentials (lse fp32 [rows][2], two parts, for _grad), and the `top` <= 32 most probable tokens with their log probabilities, the lowest id
  * first among equal logits (NaN before all).  _grad: grad [rows][vocab] contiguous, of the logits' type, from the gradients of log probability
  * and entropy (either may be null). */
 int ternaspmm_token_logprobs(const void* logits, long long ld, int type, const long long* targets, int rows, int vocab, int top,

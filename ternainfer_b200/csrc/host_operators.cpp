@@ -305,14 +305,14 @@ Scores scores_launch(const Tensor& logits, const Tensor& targets, int64_t top) {
     s.targets = targets.reshape({-1}).contiguous();
     const int64_t N = s.rows.size(0), V = s.rows.size(1);
     TORCH_CHECK_VALUE(N <= INT_MAX && V <= INT_MAX, "logits of ", logits.sizes());
-    s.stats = at::empty({3, N}, logits.options().dtype(at::kFloat));
+    s.stats = at::empty({4, N}, logits.options().dtype(at::kFloat));
     auto shape = targets.sizes().vec();
     shape.push_back(top);
     if (top) s.top_logprob = at::empty(shape, s.stats.options()), s.top_token = at::empty(shape, targets.options());
     float* stats = as<float>(s.stats);
     if (N) {
         const long long need = ternaspmm_token_logprobs_workspace((int)N, (int)V, type_code(logits), (int)top);
-        TORCH_CHECK_VALUE(need >= 0, "token_logprobs: a vocabulary of ", V, " (up to 2^20)");
+        TORCH_CHECK_VALUE(need >= 0, "token_logprobs: a vocabulary of ", V, " (up to 2^19)");
         const Tensor work = at::empty({need}, logits.options().dtype(at::kByte));   // of this call alone
         launched(ternaspmm_token_logprobs(ptr(s.rows), row_step(s.rows), type_code(logits), as<long long>(s.targets), (int)N, (int)V, (int)top, stats, stats + N,
                                           stats + 2 * N, top ? as<float>(s.top_logprob) : nullptr, top ? as<long long>(s.top_token) : nullptr, ptr(work), need,

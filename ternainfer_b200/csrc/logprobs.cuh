@@ -1,10 +1,11 @@
 // Log probabilities of given tokens for sm_100a: per row of logits the log probability of one token, the entropy of the
 // distribution and the most probable tokens, from one pass over the row; and the gradient of the first two.
 //
-// With a reference r and t = x log2(e) - r,  l = sum 2^t and w = sum 2^t t:  lse = ln(2) (r + log2 l), H = ln(2) (log2 l - w / l).
-// Rows are cut into parts of 32 KB, which a fixed number of CTAs take in turn, the next one on its way to shared memory
-// (cp.async) while one is worked on: so the load is even whatever the number of rows, and three parts per SM are always in flight.  A warp takes
-// the maximum of its share first - from shared memory, two 16-bit values at a time - and then the sums against it, so nothing
+// With a reference r and t = x log2(e) - r,  l = sum 2^t and w = sum 2^t t:  lse = ln(2) (r + log2 l), H = ln(2) (log2 l - w / l).  fp32 has room
+// for sums of elements far above the reference, so that the maximum of a run's first part serves for all of it but in the rarest cases.
+// Rows are cut into parts of 32 KB, which a fixed number of CTAs take in turn, a warp's 4 KB of the next one on their way to
+// shared memory (one bulk copy) while it works on one: so the load is even whatever the number of rows, and three parts per SM are always in flight.  A warp takes
+// the maximum of its share first - two 16-bit values at a time - and then the sums against it, so nothing
 // is ever rescaled.  For the alternatives a CTA takes up to eight parts of a row in turn: the k-th largest of the maxima of 32 groups of 8
 // threads is a bound that at least k elements of the first one reach, and few more do (k = 20: 31 on average); they and what exceeds the bound in the
 // other parts are collected, and ranked by counting.  A second kernel, a warp per row, joins the sums and merges the lists.
@@ -16,11 +17,16 @@ namespace tsp {
 
 constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32;
 constexpr int kLpVecs = 8;                                        // 16-byte vectors of a thread and part
-constexpr int kLpPartBytes = kLpThreads * kLpVecs * 16;
+constexpr int kLpPartBytes = kLpThreads * kLpVecs * 16, kLpWarpBytes = kLpPartBytes / kLpWarps;
 constexpr int kLpMaxTop = 32;
-constexpr int kLpMaxVocab = 1 << 20;
+constexpr int kLpMaxVocab = 1 << 19;
 constexpr int kLpCandidates = 512;
 constexpr int kLpCtasPerSm = 3;
+
+struct LpSums {                            // l and w relative to 2^ref
+    double ref;
+    float l, w;
+};
 
 struct LogprobParams {
     const void* logits;
@@ -29,7 +35,7 @@ struct LogprobParams {
     float *logprob, *entropy, *lse;
     float* top_logprob;                    // [rows][top]
     long long* top_token;
-    float* sums;                           // [rows][parts][warps]: r, l, w and the warp's maximum
+    LpSums* sums;                          // [rows][lists][warps]
     unsigned long long* keys;              // [rows][lists][top], largest first, 0 where there are fewer elements
     int rows, vocab, top, parts;
     int run, lists;                        // parts that a CTA takes in turn; such runs of a row
@@ -122,16 +128,17 @@ template <typename T>
 struct LpPart {
     const T* row;
     int head, vecs, first, part, parts, vocab;
-    __device__ __forceinline__ LpPart(const LogprobParams& p, long long item) {
+    __device__ __forceinline__ LpPart(const LogprobParams& p, unsigned r, int which) {
         constexpr int V = LpVec<T>::N;
-        const long long r = item / p.parts;
-        part = (int)(item - r * p.parts), parts = p.parts, vocab = p.vocab;
+        part = which, parts = p.parts, vocab = p.vocab;
         row = static_cast<const T*>(p.logits) + r * p.ld;
         head = min(vocab, (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(T));
         vecs = (vocab - head) / V, first = part * kLpThreads * kLpVecs;
     }
-    __device__ __forceinline__ int index(int j, int tid) const { return head + (first + j * kLpThreads + tid) * LpVec<T>::N; }   // of a vector's first element
-    __device__ __forceinline__ bool has(int j, int tid) const { return first + j * kLpThreads + tid < vecs; }
+    // a warp has 256 vectors behind each other, a lane every 32nd of them
+    __device__ __forceinline__ int vec(int j, int tid) const { return first + (tid >> 5) * (32 * kLpVecs) + j * 32 + (tid & 31); }
+    __device__ __forceinline__ int index(int j, int tid) const { return head + vec(j, tid) * LpVec<T>::N; }   // of a vector's first element
+    __device__ __forceinline__ bool has(int j, int tid) const { return vec(j, tid) < vecs; }
     __device__ __forceinline__ int edge(int tid) const {          // index of this thread's element of the edges, or -1
         if (part == 0 && tid < head) return tid;
         const int rest = head + vecs * LpVec<T>::N + tid - 8;
@@ -148,95 +155,132 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) logprob_kernel(const
     __shared__ uint32_t groups[32];
     __shared__ int n_cand;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t mine = smem_u32(smem) + tid * 16;
-    // run `c` of the launch is parts first .. first + count - 1 (of all rows, one behind the other)
-    const long long runs = (long long)p.rows * p.lists;
-    auto run_first = [&](long long c) { return c / p.lists * p.parts + c % p.lists * p.run; };
-    auto run_count = [&](long long c) { return min(p.run, p.parts - (int)(c % p.lists) * p.run); };
+    __shared__ __align__(8) unsigned long long bars[kLpWarps][2];
+    const uint32_t mine = smem_u32(smem) + warp * (2 * kLpWarpBytes) + lane * 16, bar = smem_u32(bars[warp]);
+    // run c of the launch: row c / lists, parts from c % lists * run on (32 bits: divisions of 64 were half of the instructions)
+    const unsigned runs = (unsigned)p.rows * (unsigned)p.lists;
     griddep_launch_dependents();
-    auto fetch = [&](long long item, int buf) {
-        const LpPart<T> at(p, item);
-#pragma unroll
-        for (int j = 0; j < kLpVecs; ++j) {
-            const uint32_t dst = mine + buf * kLpPartBytes + j * (kLpThreads * 16);
-            if (at.has(j, tid)) cp_async_16(dst, at.row + at.index(j, tid));
-            else sts128(dst, make_uint4(Vec16::none, Vec16::none, Vec16::none, Vec16::none));
+    if (lane == 0) {
+        mbar_init(bar, 1), mbar_init(bar + 8, 1);
+        mbar_fence_init();
+    }
+    __syncwarp();
+    // a warp's share of a part in one bulk copy; vectors behind the row's last one are filled in
+    auto fetch = [&](const LpPart<T>& at, int buf) {
+        const int from = at.vec(0, tid) - lane, n = min(max(at.vecs - from, 0), 32 * kLpVecs);
+        if (n < 32 * kLpVecs) {
+#pragma unroll 1
+            for (int j = 0; j < kLpVecs; ++j)
+                if (j * 32 + lane >= n) sts128(mine + buf * kLpWarpBytes + j * 512, make_uint4(Vec16::none, Vec16::none, Vec16::none, Vec16::none));
+            fence_proxy_async_smem();                              // (a later copy may write there)
+            __syncwarp();
+        }
+        if (lane == 0) {
+            mbar_arrive_expect_tx(bar + 8 * buf, n * 16);
+            if (n) bulk_load(mine + buf * kLpWarpBytes, at.row + at.index(0, tid), n * 16, bar + 8 * buf);
         }
     };
     if (tid == 0) n_cand = 0;
-    if (blockIdx.x < runs) fetch(run_first(blockIdx.x), 0);
-    cp_async_commit();
+    if (blockIdx.x < runs) fetch(LpPart<T>(p, blockIdx.x / p.lists, blockIdx.x % p.lists * p.run), 0);
+    uint32_t phases = 0;                                           // of the two barriers
+    bool ok = true;
     uint32_t bound = 0;
     int buf = 0;
 #pragma unroll 1
-    for (long long run = blockIdx.x; run < runs; run += gridDim.x) {
-    const long long first = run_first(run);
-    const int count = run_count(run);
+    for (unsigned run = blockIdx.x; run < runs; run += gridDim.x) {
+    const unsigned r_now = run / p.lists, next = run + gridDim.x;
+    const int first = (int)(run - r_now * p.lists) * p.run, count = min(p.run, p.parts - first);
     bool full = false;
+    // the warp's sums: l, w of every lane's elements, relative to 2^ref; `near`: ref is a float that takes the short way, up to elements of `limit`
+    double ref = -INFINITY;
+    float2 l = make_float2(0.f, 0.f), w = l;
+    bool near = false;
+    float limit = 0.f;
+    LpPart<T> at(p, r_now, first);
 #pragma unroll 1
-    for (int k = 0; k < count; ++k, buf ^= 1) {
-        const long long item = first + k;
-        if (k + 1 < count) fetch(item + 1, buf ^ 1);
-        else if (run + gridDim.x < runs) fetch(run_first(run + gridDim.x), buf ^ 1);
-        cp_async_commit();
-        const LpPart<T> at(p, item);
+    for (int k = 0; k < count; ++k, buf ^= 1, ++at.part, at.first += kLpThreads * kLpVecs) {
+        __syncwarp();                                              // (every lane has read what lay there)
+        if (k + 1 < count) {
+            LpPart<T> then = at;
+            ++then.part, then.first += kLpThreads * kLpVecs;
+            fetch(then, buf ^ 1);
+        } else if (next < runs) {
+            fetch(LpPart<T>(p, next / p.lists, next % p.lists * p.run), buf ^ 1);
+        }
         const int edge = at.edge(tid);
         const float xe = edge >= 0 ? Elem<T>::get(at.row[edge]) : -INFINITY;
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
-        const uint32_t src = mine + buf * kLpPartBytes;
+        ok = mbar_wait_bounded(bar + 8 * buf, phases >> buf & 1u) && ok;
+        phases ^= 1u << buf;
+        const uint32_t src = mine + buf * kLpWarpBytes;
+        Vec16 x16[kLpVecs];
         float tm = xe;                                             // this thread's maximum (NaN aside)
         uint32_t hits = 0;                                         // vectors with an element above the bound of the parts before
         const float above = k > 0 ? lp_value(bound) : INFINITY;
 #pragma unroll
+        for (int j = 0; j < kLpVecs; ++j) x16[j].w = lds128(src + j * 512);
+#pragma unroll
         for (int j = 0; j < kLpVecs; ++j) {
-            const float vm = Vec16{lds128(src + j * (kLpThreads * 16))}.max();
+            const float vm = x16[j].max();
             tm = fmaxf(tm, vm);
             if (vm > above) hits |= 1u << j;
         }
-        float m = tm;
-#pragma unroll
-        for (int j = 16; j; j >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, j));
-        float2 l = make_float2(0.f, 0.f), w = l;
-        float r = 0.f;
-        if (lp_near<T>(m)) {
-            r = m * kLog2e;
+        float2 pl = make_float2(0.f, 0.f), pw = pl;
+        auto add_all = [&](float r, float2& sl, float2& sw) {      // t = x log2(e) - r
             const float2 e2 = make_float2(kLog2e, kLog2e), nr = make_float2(-r, -r);
 #pragma unroll
             for (int j = 0; j < kLpVecs; ++j) {
                 float x[V];
-                Vec16{lds128(src + j * (kLpThreads * 16))}.floored().get(x);
+                x16[j].floored().get(x);
 #pragma unroll
                 for (int i = 0; i < V; i += 2) {
                     const float2 t = f32x2_fma(make_float2(x[i], x[i + 1]), e2, nr), e = make_float2(ex2_approx(t.x), ex2_approx(t.y));
-                    l = f32x2_add(l, e), w = f32x2_fma(e, t, w);
+                    sl = f32x2_add(sl, e), sw = f32x2_fma(e, t, sw);
                 }
             }
             if (edge >= 0) {
                 const float t = fmaf(xe < -1e37f ? -1e37f : xe, kLog2e, -r), e = ex2_approx(t);
-                l.x += e, w.x = fmaf(e, t, w.x);
+                sl.x += e, sw.x = fmaf(e, t, sw.x);
             }
-        } else {                                                   // a maximum of the type's largest or lowest order, or infinite: differences first
-            auto add = [&](float x) {
-                const float t = fmaxf((x - m) * kLog2e, -200.f), e = x == -INFINITY ? 0.f : ex2_approx((x - m) * kLog2e);
-                l.x += e, w.x = fmaf(e, t, w.x);
-            };
+        };
+        if (near && !__any_sync(0xffffffffu, tm > limit)) {
+            add_all((float)ref, pl, pw);
+            l = f32x2_add(l, pl), w = f32x2_add(w, pw);
+        } else {                                                   // the first part of a run, or one with much larger elements
+            float m = tm;
+#pragma unroll
+            for (int j = 16; j; j >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, j));
+            double part_ref = (double)m * kLog2e;
+            if (lp_near<T>(m)) {
+                part_ref = m * kLog2e;                             // (as rounded to fp32)
+                add_all((float)part_ref, pl, pw);
+            } else {                                               // a maximum of the type's largest or lowest order, or infinite: differences first
+                auto add = [&](float x) {
+                    const float t = fmaxf((x - m) * kLog2e, -200.f), e = x == -INFINITY ? 0.f : ex2_approx((x - m) * kLog2e);
+                    pl.x += e, pw.x = fmaf(e, t, pw.x);
+                };
 #pragma unroll 1
-            for (int j = 0; j < kLpVecs; ++j) {
-                float x[V];
-                Vec16{lds128(src + j * (kLpThreads * 16))}.get(x);
+                for (int j = 0; j < kLpVecs; ++j) {
+                    float x[V];
+                    Vec16{lds128(src + j * 512)}.get(x);
 #pragma unroll
-                for (int i = 0; i < V; ++i) add(x[i]);
+                    for (int i = 0; i < V; ++i) add(x[i]);
+                }
+                if (edge >= 0) add(xe);
             }
-            if (edge >= 0) add(xe);
+            // (part_ref of -inf: nothing but -inf and NaN)
+            const double to = fmax(ref, part_ref);
+            const float ds = ref == -INFINITY ? 0.f : (float)(ref - to), dp = part_ref == -INFINITY ? 0.f : (float)(part_ref - to);
+            const float fs = ex2_approx(ds), fp = ex2_approx(dp), cs = fmaxf(ds, -200.f), cp = fmaxf(dp, -200.f);
+            w.x = (w.x + w.y + (l.x + l.y) * cs) * fs + (pw.x + pw.y + (pl.x + pl.y) * cp) * fp, w.y = 0.f;
+            l.x = (l.x + l.y) * fs + (pl.x + pl.y) * fp, l.y = 0.f;
+            ref = to;
+            near = fabs(ref) < 1.4e36 && lp_near<T>((float)(ref * 0.69314718)) && (double)(float)ref == ref;
+            limit = (float)((ref + 60) * 0.69314718);              // (2^60 times as many elements as a row has fit into fp32)
         }
-        l.x += l.y, w.x += w.y;
-        const float own = l.x;
-#pragma unroll
-        for (int j = 16; j; j >>= 1) l.x += __shfl_xor_sync(0xffffffffu, l.x, j), w.x += __shfl_xor_sync(0xffffffffu, w.x, j);
-        if (lane == 0) *reinterpret_cast<float4*>(p.sums + (item * kLpWarps + warp) * 4) = make_float4(r, l.x, w.x, m);
         if (p.top == 0) continue;
 
         // ---- candidates for the most probable tokens
+        const float own = pl.x + pl.y;
         const bool odd = own != own;                               // NaN or +inf among this thread's elements: which, the sum does not tell
         if (k == 0) {
             uint32_t u = lp_order(tm);
@@ -245,7 +289,7 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) logprob_kernel(const
 #pragma unroll 1
                 for (int j = 0; j < kLpVecs; ++j) {
                     float x[V];
-                    Vec16{lds128(src + j * (kLpThreads * 16))}.get(x);
+                    Vec16{lds128(src + j * 512)}.get(x);
 #pragma unroll
                     for (int i = 0; i < V; ++i) u = max(u, lp_order(x[i]));
                 }
@@ -256,15 +300,18 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) logprob_kernel(const
             if ((lane & 7) == 0) groups[warp * 4 + (lane >> 3)] = gm;
             __syncthreads();
             const uint32_t v = groups[lane];
-            bound = 0;
-#pragma unroll 1
-            for (uint32_t bit = 0x80000000u; bit; bit >>= 1)       // the largest that p.top of the groups reach
-                if (__popc(__ballot_sync(0xffffffffu, v >= (bound | bit))) >= p.top) bound |= bit;
+            int rank = 0;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+                const uint32_t other = __shfl_sync(0xffffffffu, v, j);
+                rank += other > v || (other == v && j < lane);
+            }
+            bound = __shfl_sync(0xffffffffu, v, __ffs(__ballot_sync(0xffffffffu, rank == p.top - 1)) - 1);   // that p.top of the groups reach
             if (u >= bound) {
                 const float bf = lp_value(bound);
 #pragma unroll
                 for (int j = 0; j < kLpVecs; ++j)
-                    if (!(Vec16{lds128(src + j * (kLpThreads * 16))}.max() < bf)) hits |= 1u << j;
+                    if (!(x16[j].max() < bf)) hits |= 1u << j;
             }
         }
         if (odd && bound != 0xffffffffu) hits = (1u << kLpVecs) - 1;
@@ -283,39 +330,50 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) logprob_kernel(const
             hits &= hits - 1;
             if (!at.has(j, tid)) continue;
             float x[V];
-            Vec16{lds128(src + j * (kLpThreads * 16))}.get(x);
+            Vec16{lds128(src + j * 512)}.get(x);
 #pragma unroll
             for (int i = 0; i < V; ++i)
                 if (!(x[i] < bf)) push(x[i], at.index(j, tid) + i);
         }
         if (edge >= 0 && !(bound == 0xffffffffu && k > 0)) push(xe, edge);
-        // ---- after the parts 1, 2, 4 of a run and its last one the best are kept, in their order, and the bound follows
-        if (k == 0 || k == 1 || k == 3 || k == count - 1) {
+        // ---- after the parts 1 and 3 of a run and its last one the best are kept, in their order, and the bound follows
+        if (k == 0 || k == 2 || k == count - 1) {
             __syncthreads();
             const int n = n_cand;
             if (n > kLpCandidates) {                               // many elements at the bound or above it: found at the end
                 full = true, bound = 0xffffffffu;
             } else {
-                unsigned long long key[kLpCandidates / kLpThreads];
-                int rank[kLpCandidates / kLpThreads];
+                constexpr int PER = kLpThreads / 4;                // four threads to a candidate
+                unsigned long long key[kLpCandidates / PER];
+                int rank[kLpCandidates / PER];
 #pragma unroll
-                for (int i = 0; i < kLpCandidates / kLpThreads; ++i) {
-                    key[i] = tid + i * kLpThreads < n ? cand[tid + i * kLpThreads] : 0ull, rank[i] = 0;
-                    if (key[i])
-                        for (int j = 0; j < n; ++j) rank[i] += cand[j] > key[i];
+                for (int i = 0; i < kLpCandidates / PER; ++i) {
+                    const int c = i * PER + (tid >> 2);
+                    key[i] = 0ull, rank[i] = 0;
+                    if (i * PER >= n) continue;                    // (the same for all threads)
+                    key[i] = c < n ? cand[c] : 0ull;
+                    for (int j = tid & 3; j < n; j += 4) rank[i] += cand[j] > key[i];
+                    rank[i] += __shfl_xor_sync(0xffffffffu, rank[i], 1);
+                    rank[i] += __shfl_xor_sync(0xffffffffu, rank[i], 2);
                 }
                 __syncthreads();
 #pragma unroll
-                for (int i = 0; i < kLpCandidates / kLpThreads; ++i)
-                    if (key[i] && rank[i] < p.top) cand[rank[i]] = key[i];
+                for (int i = 0; i < kLpCandidates / PER; ++i)
+                    if ((tid & 3) == 0 && key[i] && rank[i] < p.top) cand[rank[i]] = key[i];
                 if (tid == 0) n_cand = min(n, p.top);
                 __syncthreads();
                 if (n >= p.top) bound = (uint32_t)(cand[p.top - 1] >> 32);
             }
         }
     }
+    {
+        float sl = l.x + l.y, sw = w.x + w.y;
+#pragma unroll
+        for (int j = 16; j; j >>= 1) sl += __shfl_xor_sync(0xffffffffu, sl, j), sw += __shfl_xor_sync(0xffffffffu, sw, j);
+        if (lane == 0) p.sums[(size_t)run * kLpWarps + warp] = {ref, ok ? sl : __int_as_float(0x7fffffff), sw};
+    }
     if (p.top == 0) continue;
-    unsigned long long* keys = p.keys + run * p.top;
+    unsigned long long* keys = p.keys + (size_t)run * p.top;
     if (!full) {
         if (tid < p.top) keys[tid] = tid < n_cand ? cand[tid] : 0ull;
     } else {                                                       // a pass over the run for each place
@@ -328,7 +386,7 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) logprob_kernel(const
             };
 #pragma unroll 1
             for (int k = 0; k < count; ++k) {
-                const LpPart<T> at(p, first + k);
+                const LpPart<T> at(p, r_now, first + k);
 #pragma unroll 1
                 for (int j = 0; j < kLpVecs; ++j) {
                     if (!at.has(j, tid)) continue;
@@ -357,11 +415,13 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) logprob_kernel(const
     __syncthreads();
     if (tid == 0) n_cand = 0;                                      // (seen by all at the next run's first barrier)
     }
+    if (!ok && lane == 0) atomicExch(p.status, ST_WAIT_TIMEOUT);
 }
 
-// Log probability; rounding does not take it above 0.
-__device__ __forceinline__ float lp_least(float x, float m, float ln) {
-    const float lp = (x - m) - ln;
+// Log probability of x beside a sum of 2^(ref + ll) (differences first: ll is nothing beside the reference of a row of the type's lowest value);
+// rounding does not take it above 0.
+__device__ __forceinline__ float lp_of(float x, double ref, float ll) {
+    const float lp = (float)((((double)x * (double)kLog2e - ref) - ll) / (double)kLog2e);
     return lp > 0.f ? 0.f : lp;
 }
 
@@ -375,32 +435,27 @@ __global__ void __launch_bounds__(32) logprob_join_kernel(const LogprobParams p)
     const long long target = p.targets[r];
     const float xt = target >= 0 && target < p.vocab ? Elem<T>::get(row[target]) : 0.f;
     griddep_wait();
-    const float4* s = reinterpret_cast<const float4*>(p.sums) + r * p.parts * kLpWarps;
-    const int n = p.parts * kLpWarps;
+    const LpSums* s = p.sums + r * p.lists * kLpWarps;
+    const int n = p.lists * kLpWarps;
     int* place = reinterpret_cast<int*>(lists + p.lists * p.top);
     for (int i = lane; i < p.lists * p.top; i += 32) lists[i] = p.keys[r * p.lists * p.top + i];
     for (int i = lane; i < p.lists; i += 32) place[i] = 0;
-    float m = -INFINITY, l = 0.f, w = 0.f;
-    for (int i = lane; i < n; i += 32) m = fmaxf(m, s[i].w);
+    double ref = -INFINITY;
+    float l = 0.f, w = 0.f;
+    for (int i = lane; i < n; i += 32) ref = fmax(ref, s[i].ref);
 #pragma unroll
-    for (int j = 16; j; j >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, j));
-    // the warps' sums are relative to r = m log2(e) as rounded, or to m itself where that is far out
-    const bool far = !lp_near<T>(m);
-    const float ref = far ? 0.f : m * kLog2e;
+    for (int j = 16; j; j >>= 1) ref = fmax(ref, __shfl_xor_sync(0xffffffffu, ref, j));
     for (int i = lane; i < n; i += 32) {
-        const float4 a = s[i];
-        // exponent that takes the warp's sums to the row's reference
-        const float d = a.w == -INFINITY ? (a.y != a.y ? 0.f : -INFINITY) : far ? (a.w - m) * kLog2e : lp_near<T>(a.w) ? a.x - ref : fmaf(a.w, kLog2e, -ref);
-        const float f = ex2_approx(d);
-        l += a.y * f, w += (a.z + a.y * fmaxf(d, -200.f)) * f;
+        const LpSums a = s[i];
+        const float d = a.ref == -INFINITY ? 0.f : (float)(a.ref - ref), f = ex2_approx(d);   // (-inf: l is 0 or NaN)
+        l += a.l * f, w += (a.w + a.l * fmaxf(d, -200.f)) * f;
     }
 #pragma unroll
     for (int j = 16; j; j >>= 1) l += __shfl_xor_sync(0xffffffffu, l, j), w += __shfl_xor_sync(0xffffffffu, w, j);
-    const float ll = log2f(l);
-    // ln of the sum of exp(x - m); m log2(e) was rounded
-    const float ln = m == -INFINITY ? __int_as_float(0x7fffffff) : far ? ll * kLn2 : (ll - fmaf(m, kLog2e, -ref)) * kLn2;
+    // log2 of the sum of 2^(x log2(e)); the units are those of log2(e) as rounded to fp32.  Without a finite logit it is NaN
+    const float ll = ref == -INFINITY ? __int_as_float(0x7fffffff) : log2f(l);
     if (lane == 0) {
-        float lp = lp_least(xt, m, ln);
+        float lp = lp_of(xt, ref, ll);
         if (target < 0) lp = 0.f;                                  // no token
         if (target >= p.vocab) {
             lp = __int_as_float(0x7fffffff);
@@ -408,8 +463,10 @@ __global__ void __launch_bounds__(32) logprob_join_kernel(const LogprobParams p)
         }
         p.logprob[r] = lp;
         const float h = (ll - w / l) * kLn2;
-        p.entropy[r] = ln != ln ? ln : h < 0.f ? 0.f : h;
-        p.lse[r] = m + ln;
+        p.entropy[r] = h < 0.f ? 0.f : h;
+        // in two parts, for the gradient
+        const float hi = (float)(ref / (double)kLog2e);
+        p.lse[2 * r] = hi, p.lse[2 * r + 1] = (float)(((ref - (double)hi * (double)kLog2e) + ll) / (double)kLog2e);
     }
     __syncwarp();
     for (int k = 0; k < p.top; ++k) {                              // the lists' heads against each other
@@ -427,7 +484,7 @@ __global__ void __launch_bounds__(32) logprob_join_kernel(const LogprobParams p)
         }
         if (key == top) {                                          // (keys differ: one lane; top <= vocab: none is 0)
             ++place[from];
-            p.top_logprob[r * p.top + k] = lp_least(lp_value((uint32_t)(key >> 32)), m, ln);
+            p.top_logprob[r * p.top + k] = lp_of(lp_value((uint32_t)(key >> 32)), ref, ll);
             p.top_token[r * p.top + k] = 0xffffffffu - (uint32_t)key;
         }
         __syncwarp();
@@ -453,9 +510,9 @@ __global__ void __launch_bounds__(256) logprob_grad_kernel(const LogprobGradPara
     T* out = static_cast<T*>(p.grad) + r * (size_t)p.vocab;
     const long long t = p.targets[r];
     const float g = p.g_logprob && t >= 0 ? p.g_logprob[r] : 0.f, h = p.g_entropy ? p.g_entropy[r] : 0.f;
-    const float lse = p.lse[r], ent = p.entropy[r];
+    const float hi = p.lse[2 * r], lo = p.lse[2 * r + 1], ent = p.entropy[r];
     auto one = [&](int j, float x) {
-        const float lp = x - lse, e = ex2_approx(lp * kLog2e);
+        const float lp = (x - hi) - lo, e = ex2_approx(lp * kLog2e);
         const float d = -e * fmaf(h, fmaxf(lp, -200.f) + ent, g);
         return j == t ? d + g : d;
     };

@@ -1388,12 +1388,12 @@ static int logprob_parts(int vocab, int type) {
     return (vocab + part - 1) / part;
 }
 static bool logprob_shape(int rows, int vocab, int type, int top) {
-    return rows >= 1 && vocab >= 1 && vocab <= kLpMaxVocab && type >= 0 && type <= 2 && top >= 0 && top <= kLpMaxTop && top <= vocab;
+    return rows >= 1 && rows <= (1 << 23) && vocab >= 1 && vocab <= kLpMaxVocab && type >= 0 && type <= 2 && top >= 0 && top <= kLpMaxTop && top <= vocab;
 }
 
 extern "C" long long ternaspmm_token_logprobs_workspace(int rows, int vocab, int type, int top) {
     if (!logprob_shape(rows, vocab, type, top)) return -1;
-    return (long long)rows * logprob_parts(vocab, type) * (kLpWarps * 16 + 8 * top);
+    return (long long)rows * logprob_parts(vocab, type) * (kLpWarps * (int)sizeof(LpSums) + 8 * top);
 }
 
 template <typename T>
@@ -1433,13 +1433,12 @@ extern "C" int ternaspmm_token_logprobs(const void* logits, long long ld, int ty
     t_host_status = ST_OK;
     if (!logprob_shape(rows, vocab, type, top) || ld < vocab || workspace_bytes < ternaspmm_token_logprobs_workspace(rows, vocab, type, top))
         return t_host_status = ST_BAD_SHAPE;
-    LogprobParams p = {logits, ld, targets, logprob, entropy, lse, top_logprob, top_token, static_cast<float*>(workspace), nullptr, rows, vocab, top,
+    LogprobParams p = {logits, ld, targets, logprob, entropy, lse, top_logprob, top_token, static_cast<LpSums*>(workspace), nullptr, rows, vocab, top,
                        logprob_parts(vocab, type), 1, 1, status_device_ptr()};
-    // up to eight parts of a row in turn, as long as every CTA has at least two such runs (one where the alternatives are not asked for: nothing
-    // is carried from part to part then)
-    if (top) p.run = (int)std::max(1ll, std::min(8ll, (long long)rows * p.parts / (2ll * kLpCtasPerSm * device_sm_count())));
+    // up to eight parts of a row in turn, as long as every CTA has at least two such runs
+    p.run = (int)std::max(1ll, std::min(8ll, (long long)rows * p.parts / (2ll * kLpCtasPerSm * device_sm_count())));
     p.lists = (p.parts + p.run - 1) / p.run;
-    p.keys = reinterpret_cast<unsigned long long*>(p.sums + (size_t)rows * p.parts * kLpWarps * 4);
+    p.keys = reinterpret_cast<unsigned long long*>(p.sums + (size_t)rows * p.lists * kLpWarps);
     if (!logits || !targets || !logprob || !entropy || !lse || !workspace || (top && (!top_logprob || !top_token)) ||
         reinterpret_cast<uintptr_t>(logits) % (type == 2 ? 4 : 2) || (reinterpret_cast<uintptr_t>(workspace) & 15))
         return t_host_status = ST_BAD_POINTER;

@@ -38,7 +38,7 @@ def check(x, t, top):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("N,V", [(1, 1), (3, 2), (2, 7), (5, 33), (1, 511), (2, 512), (3, 513), (2, 1000), (7, 2049), (2, 4097), (300, 777), (3, 32000), (2, 128256), (1, 250001), (1, 1 << 20), (700, 20011)])
+@pytest.mark.parametrize("N,V", [(1, 1), (3, 2), (2, 7), (5, 33), (1, 511), (2, 512), (3, 513), (2, 1000), (7, 2049), (2, 4097), (300, 777), (3, 32000), (2, 128256), (1, 250001), (1, 1 << 19), (700, 20011)])
 def test_logprobs(lib, dtype, N, V):
     g = gen(V)
     x = (3 * torch.randn((N, V), generator=g, device="cuda")).to(dtype)
@@ -147,6 +147,22 @@ def test_gradient(lib, dtype, N, V):
         got, = torch.autograd.grad(f(leaf), leaf)
         slope = (f(x + e * d) - f(x - e * d)) / (2 * e)
         assert abs(slope - (got.double() * d.double()).sum()) < 2e-2 * got.double().norm() * d.double().norm() / V ** 0.5
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradient_of_fully_masked_rows(lib, dtype):
+    """Rows of the type's lowest value alone are uniform, and so is their gradient; a row of -inf alone has none (NaN), its neighbours theirs."""
+    V = 9000
+    x = torch.full((3, V), torch.finfo(dtype).min, dtype=dtype, device="cuda")
+    x[1], x[2, ::3] = float("-inf"), 5.0
+    leaf = x.requires_grad_()
+    r = token_logprobs(leaf, torch.full((3,), 6, device="cuda"))
+    got, = torch.autograd.grad(r.logprob.sum(), leaf)
+    want = -torch.stack([torch.full((V,), 1 / V), torch.full((V,), float("nan")), (torch.arange(V) % 3 == 0) * (3 / V)]).cuda().double()
+    want[:, 6] += 1
+    assert torch.equal(got.isnan(), want.isnan())
+    # one exponential of ln V, in fp32: 2^-20 relative; then a rounding
+    assert ((got.double() - want).nan_to_num(0).abs() <= want.nan_to_num(0).abs() * (2.0 ** -20 + torch.finfo(dtype).eps / 2) + torch.finfo(dtype).tiny).all()
 
 
 def test_gradient_of_strided_and_broadcast_rows(lib):
