@@ -349,7 +349,7 @@ int ternaspmm_rotate(const void* q, const long long* q_strides, int q_heads, voi
  * how many of them there are (null: all).  Sequences whose tokens do not fit into the cache are refused as a whole.
  *
  * _append: rotates q (may be null; then no q_out) and k by position where tables are given (bf16 results, ternaspmm_rotate's
- * arithmetic) and writes the rows start .. start + count - 1.  8-byte aligned pointers, strides multiples of 4.
+ * arithmetic) and writes the rows start .. start + count - 1.  8-byte aligned inputs, strides multiples of 4; results 16-byte aligned.
  * _read: the values that rows stand for, bf16 [batch][tokens][kv_heads][head_dim]; zeros behind a sequence's count. */
 int ternaspmm_kv4_append(void* k_codes, void* k_scales, void* v_codes, void* v_scales, int max_len, const ternaspmm_bf16* k,
                          const long long* k_strides, const ternaspmm_bf16* v, const long long* v_strides, const ternaspmm_bf16* q,

@@ -35,7 +35,9 @@ struct Kv4AppendParams {
     const float *cos_tab, *sin_tab;        // null: no rotation
     const long long *start, *counts;       // position of the first new token; new tokens (null: all)
     int start_stride;                      // 0: the same for every sequence
-    int tokens, heads, rotary, half, table_len;
+    FastDiv head_groups, tokens;
+    int heads, rotary, half, table_len;
+    int tables_16, rows_16;                // whether every table row, and every row of q, k and v, starts on 16 bytes
     int* status;
 };
 
@@ -44,113 +46,204 @@ __device__ __forceinline__ bool kv4_fits(long long start, long long count, int t
     return start >= 0 && count >= 0 && count <= tokens && start <= max_len && start + count <= max_len;
 }
 
-// One row (head of a token) per D / 4 lanes, 4 values a lane.  Rows: queries (rotated into q_out), keys (rotated, quantised),
-// values (quantised).
+// Where 8 consecutive values of a row of codes lie, `u` the unit of 8: one word of a key row, two halfwords of a value row.
 template <int D>
-__global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4AppendParams p, long long rows) {
-    constexpr int LANES = D / 4;
-    const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) / LANES;
-    const int lane = threadIdx.x % LANES, e = lane * 4;
-    const bool live = r < rows;                                    // (all lanes take part in the shuffles)
-    const int kv = p.c.kv_heads, per_token = (p.q.x ? p.heads : 0) + 2 * kv;
-    const long long bt = live ? r / per_token : 0, b = bt / p.tokens, t = bt - b * p.tokens;
-    int h = live ? (int)(r - bt * per_token) : 0;
-    const bool is_q = p.q.x && h < p.heads;
-    if (!is_q && p.q.x) h -= p.heads;
-    const bool is_k = !is_q && h < kv;
-    if (!is_q && !is_k) h -= kv;
-    const Kv4Side& sd = is_q ? p.q : is_k ? p.k : p.v;
-    const __nv_bfloat16* src = sd.x + b * sd.sb + t * sd.st + h * sd.sh;
-    const long long start = p.start[b * p.start_stride], count = p.counts ? p.counts[b] : p.tokens;
-    const bool fits = kv4_fits(start, count, p.tokens, p.c.max_len);
-    const long long pos = start + t;
-    if (!fits && live) *p.status = 1;
-
-    const uint2 raw = *reinterpret_cast<const uint2*>(src + e);
-    float x[4] = {bf16_lo(raw.x), bf16_hi(raw.x), bf16_lo(raw.y), bf16_hi(raw.y)};
-    if (p.cos_tab && (is_q || is_k)) {
-        const int half = p.rotary / 2;
-        const bool ok = pos >= 0 && pos < p.table_len;
-        // a padded query lies behind the table at most where the cache ends: it takes NaN, and is nobody's concern
-        if (live && fits && t < count && !ok) *p.status = 1;
-        const float* ct = p.cos_tab + (ok ? pos : 0) * half;
-        const float* st = p.sin_tab + (ok ? pos : 0) * half;
-        float y[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int d = e + i;
-            y[i] = x[i];
-            if (d >= p.rotary) continue;
-            const bool first = p.half ? d < half : !(d & 1);       // of its pair
-            const int pair = p.half ? (first ? d : d - half) : d >> 1;
-            const float other = p.half ? __bfloat162float(src[first ? d + half : d - half]) : x[i ^ 1];
-            const float c = ok ? ct[pair] : __int_as_float(0x7fffffff), s = ok ? st[pair] : c;
-            y[i] = first ? rot_a(x[i], other, c, s) : rot_b(other, x[i], c, s);
-        }
-        const uint32_t lo = bf16_pack(y[0], y[1]), hi = bf16_pack(y[2], y[3]);   // rounded as the activations are
-        x[0] = bf16_lo(lo), x[1] = bf16_hi(lo), x[2] = bf16_lo(hi), x[3] = bf16_hi(hi);
-    }
-    if (is_q) {
-        if (live) *reinterpret_cast<uint2*>(p.q_out + (bt * p.heads + h) * D + e) = make_uint2(bf16_pack(x[0], x[1]), bf16_pack(x[2], x[3]));
-    }
-    float hi = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), lo = fminf(fminf(x[0], x[1]), fminf(x[2], x[3]));
-    bool nan = x[0] != x[0] || x[1] != x[1] || x[2] != x[2] || x[3] != x[3];
-#pragma unroll
-    for (int m = 1; m < 8; m <<= 1) {
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, m));
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, m));
-        nan |= __shfl_xor_sync(0xffffffffu, (int)nan, m) != 0;
-    }
-    if (!live || is_q || !fits || t >= count) return;
-    const __half scale = nan ? __ushort_as_half(0x7fff) : __float2half_rn((hi >= -lo ? hi : lo) * -0.125f);   // (a NaN stays one)
-    const float s = __half2float(scale);
-    uint32_t code = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float c = s == 0.f ? 8.f : fminf(fmaxf(rintf(__fdiv_rn(x[i], s)) + 8.f, 0.f), 15.f);
-        code |= (uint32_t)c << (4 * i);
-    }
+__device__ __forceinline__ void kv4_put_codes(uint8_t* row, bool key, int u, uint32_t codes) {
     constexpr int G = D / kKv4Group;
-    const int i = lane >> 3, g = lane & 7;
-    const size_t row = ((size_t)b * kv + h) * p.c.max_len + pos;
-    uint8_t* codes = (is_k ? p.c.k_codes : p.c.v_codes) + row * (D / 2);
-    const int at = is_k ? ((g >> 1) * G + i) * 4 + (g & 1) * 2 : (g * G + i) * 2;
-    *reinterpret_cast<uint16_t*>(codes + at) = (uint16_t)code;
-    if (g == 0) (is_k ? p.c.k_scales : p.c.v_scales)[row * G + i] = scale;
+    const int i = u >> 2, t = u & 3;
+    if (key) {
+        *reinterpret_cast<uint32_t*>(row + (t * G + i) * 4) = codes;
+    } else {
+        *reinterpret_cast<uint16_t*>(row + (2 * t * G + i) * 2) = (uint16_t)codes;
+        *reinterpret_cast<uint16_t*>(row + ((2 * t + 1) * G + i) * 2) = (uint16_t)(codes >> 16);
+    }
+}
+template <int D>
+__device__ __forceinline__ uint32_t kv4_get_codes(const uint8_t* row, bool key, int u) {
+    constexpr int G = D / kKv4Group;
+    const int i = u >> 2, t = u & 3;
+    if (key) return *reinterpret_cast<const uint32_t*>(row + (t * G + i) * 4);
+    return (uint32_t)*reinterpret_cast<const uint16_t*>(row + (2 * t * G + i) * 2) |
+           (uint32_t)*reinterpret_cast<const uint16_t*>(row + ((2 * t + 1) * G + i) * 2) << 16;
+}
+
+constexpr int kKv4Heads = 4;               // rows of a token that a thread of the reading kernel takes a unit of
+
+// A thread takes 8 consecutive values in HEADS heads of a token - queries (rotated into q_out), keys (rotated, quantised), values
+// (quantised) -, all of them on their way before the first is used; four lanes share a group's scale.
+template <int D, int HEADS>
+__global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4AppendParams p, uint32_t items) {
+    constexpr int U = D / 8, G = D / kKv4Group;
+    const uint32_t item = blockIdx.x * 256u + threadIdx.x;
+    const bool live = item < items;                                // (all lanes take part in the shuffles)
+    const int u = item % U, e = u * 8, kv = p.c.kv_heads;
+    uint32_t hg, t;
+    const uint32_t bt = p.head_groups.div(live ? item / U : 0u, hg), b = p.tokens.div(bt, t);
+    const long long start = p.start[(long long)b * p.start_stride], count = p.counts ? p.counts[b] : (long long)p.tokens.d;
+    const bool fits = kv4_fits(start, count, (int)p.tokens.d, p.c.max_len);
+    if (!fits && live) *p.status = 1;
+    const long long pos = start + t;
+    const int half = p.rotary / 2;
+    const bool turns = p.cos_tab && e < p.rotary, pos_ok = pos >= 0 && pos < p.table_len;
+    // a padded query behind the table takes NaN, and is nobody's concern
+    if (turns && live && fits && t < count && !pos_ok) *p.status = 1;
+    // pairs of 8 values whose other halves are 8 values too, or neighbours: whole vectors
+    const bool whole = p.half ? half % 8 == 0 : p.rotary % 8 == 0, second = p.half && e >= half;
+    uint4 x[HEADS], y[HEADS];
+    int kind[HEADS], head[HEADS];                          // 0 query, 1 key, 2 value
+#pragma unroll
+    for (int i = 0; i < HEADS; ++i) {
+        const int h = (int)hg * HEADS + i;
+        kind[i] = h < p.heads ? 0 : h < p.heads + kv ? 1 : h < p.heads + 2 * kv ? 2 : 3;
+        head[i] = kind[i] == 0 ? h : kind[i] == 1 ? h - p.heads : h - p.heads - kv;
+        x[i] = y[i] = make_uint4(0, 0, 0, 0);
+        if (!live || kind[i] == 3) continue;
+        const Kv4Side& sd = kind[i] == 0 ? p.q : kind[i] == 1 ? p.k : p.v;
+        const __nv_bfloat16* src = sd.x + (long long)b * sd.sb + (long long)t * sd.st + (long long)head[i] * sd.sh;
+        if (p.rows_16) {
+            x[i] = ld_cg_128(src + e);
+            if (turns && p.half && whole && kind[i] < 2) y[i] = ld_cg_128(src + (second ? e - half : e + half));
+        } else {
+            const uint2 lo = *reinterpret_cast<const uint2*>(src + e), hi = *reinterpret_cast<const uint2*>(src + e + 4);
+            x[i] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+            if (turns && p.half && whole && kind[i] < 2) {
+                const __nv_bfloat16* o = src + (second ? e - half : e + half);
+                const uint2 olo = *reinterpret_cast<const uint2*>(o), ohi = *reinterpret_cast<const uint2*>(o + 4);
+                y[i] = make_uint4(olo.x, olo.y, ohi.x, ohi.y);
+            }
+        }
+    }
+    float c[8], s[8];
+    if (turns && whole) {
+        const long long row = (pos_ok ? pos : 0) * half;
+        if (p.half) {
+            table_values(p.cos_tab + row + (second ? e - half : e), p.tables_16, c);
+            table_values(p.sin_tab + row + (second ? e - half : e), p.tables_16, s);
+        } else {
+            float c4[4], s4[4];
+            table_values(p.cos_tab + row + e / 2, p.tables_16, c4);
+            table_values(p.sin_tab + row + e / 2, p.tables_16, s4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) c[j] = c4[j], s[j] = s4[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) c[j] = pos_ok ? c[j] : __int_as_float(0x7fffffff);
+    }
+#pragma unroll
+    for (int i = 0; i < HEADS; ++i) {
+        float v[8];
+        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[2 * j] = bf16_lo(w[j]), v[2 * j + 1] = bf16_hi(w[j]);
+        if (turns && kind[i] < 2 && live) {
+            float r[8];
+            if (whole && p.half) {
+                const uint32_t o[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float other = j & 1 ? bf16_hi(o[j >> 1]) : bf16_lo(o[j >> 1]);
+                    r[j] = second ? rot_b(other, v[j], c[j], s[j]) : rot_a(v[j], other, c[j], s[j]);
+                }
+            } else if (whole) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) r[2 * j] = rot_a(v[2 * j], v[2 * j + 1], c[j], s[j]), r[2 * j + 1] = rot_b(v[2 * j], v[2 * j + 1], c[j], s[j]);
+            } else {                                               // the rotated part ends, or changes sides, inside of the 8 values
+                const Kv4Side& sd = kind[i] == 0 ? p.q : p.k;
+                const __nv_bfloat16* src = sd.x + (long long)b * sd.sb + (long long)t * sd.st + (long long)head[i] * sd.sh;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int d = e + j;
+                    r[j] = v[j];
+                    if (d >= p.rotary) continue;
+                    const bool first = p.half ? d < half : !(d & 1);   // of its pair
+                    const int pair = p.half ? (first ? d : d - half) : d >> 1;
+                    const float other = p.half ? __bfloat162float(src[first ? d + half : d - half]) : v[j ^ 1];
+                    const float cc = pos_ok ? p.cos_tab[pos * half + pair] : __int_as_float(0x7fffffff), ss = pos_ok ? p.sin_tab[pos * half + pair] : cc;
+                    r[j] = first ? rot_a(v[j], other, cc, ss) : rot_b(other, v[j], cc, ss);
+                }
+            }
+            x[i] = make_uint4(bf16_pack(r[0], r[1]), bf16_pack(r[2], r[3]), bf16_pack(r[4], r[5]), bf16_pack(r[6], r[7]));   // rounded as the activations are
+            const uint32_t z[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[2 * j] = bf16_lo(z[j]), v[2 * j + 1] = bf16_hi(z[j]);
+        }
+        if (kind[i] == 0 && live) *reinterpret_cast<uint4*>(p.q_out + ((long long)bt * p.heads + head[i]) * D + e) = x[i];
+        // (a half-warp or quarter has one head: its lanes go the same way up to here but for `live`)
+        float hi = v[0], lo = v[0];
+        bool nan = v[0] != v[0];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) hi = fmaxf(hi, v[j]), lo = fminf(lo, v[j]), nan |= v[j] != v[j];
+#pragma unroll
+        for (int m = 1; m < 4; m <<= 1) {
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, m));
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, m));
+            nan |= __shfl_xor_sync(0xffffffffu, (int)nan, m) != 0;
+        }
+        if (!live || kind[i] == 0 || kind[i] == 3 || !fits || t >= count) continue;
+        const __half scale = nan ? __ushort_as_half(0x7fff) : __float2half_rn((hi >= -lo ? hi : lo) * -0.125f);   // (a NaN stays one)
+        const float sc = __half2float(scale), inv = __frcp_rn(sc);
+        uint32_t code = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            // a product with the reciprocal is within 2^-19 of the quotient; where that may matter the quotient decides
+            const float t = v[j] * inv;
+            float q = rintf(t);
+            if (fabsf(t - q) > 0.4999f) q = rintf(__fdiv_rn(v[j], sc));
+            q = sc == 0.f ? 8.f : fminf(fmaxf(q + 8.f, 0.f), 15.f);
+            code |= (uint32_t)q << (4 * j);
+        }
+        const size_t row = ((size_t)b * kv + head[i]) * p.c.max_len + pos;
+        kv4_put_codes<D>((kind[i] == 1 ? p.c.k_codes : p.c.v_codes) + row * (D / 2), kind[i] == 1, u, code);
+        if ((u & 3) == 0) (kind[i] == 1 ? p.c.k_scales : p.c.v_scales)[row * G + (u >> 2)] = scale;
+    }
 }
 
 struct Kv4ReadParams {
     Kv4Cache c;
     __nv_bfloat16 *k_out, *v_out;          // [B][T][Hkv][D]
     const long long *start, *counts;
-    int start_stride, tokens;
+    int start_stride;
+    FastDiv head_groups, tokens;
     int* status;
 };
 
 template <int D>
-__global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p, long long rows) {
-    constexpr int LANES = D / 4, G = D / kKv4Group;
-    const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) / LANES;
-    if (r >= rows) return;
-    const int lane = threadIdx.x % LANES, kv = p.c.kv_heads, hk = (int)(r % (2 * kv)), i = lane >> 3, g = lane & 7;
-    const long long bt = r / (2 * kv), b = bt / p.tokens, t = bt - b * p.tokens;
-    const bool is_k = hk < kv;
-    const int h = is_k ? hk : hk - kv;
-    const long long start = p.start[b * p.start_stride], count = p.counts ? p.counts[b] : p.tokens;
-    const bool fits = kv4_fits(start, count, p.tokens, p.c.max_len);
-    float x[4] = {0.f, 0.f, 0.f, 0.f};
-    if (!fits) {
-        x[0] = x[1] = x[2] = x[3] = __int_as_float(0x7fffffff);
-        *p.status = 1;
-    } else if (t < count) {
-        const size_t row = ((size_t)b * kv + h) * p.c.max_len + start + t;
-        const int at = is_k ? ((g >> 1) * G + i) * 4 + (g & 1) * 2 : (g * G + i) * 2;
-        const uint32_t code = *reinterpret_cast<const uint16_t*>((is_k ? p.c.k_codes : p.c.v_codes) + row * (D / 2) + at);
-        const float s = __half2float((is_k ? p.c.k_scales : p.c.v_scales)[row * G + i]);
+__global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p, uint32_t items) {
+    constexpr int U = D / 8, G = D / kKv4Group;
+    const uint32_t item = blockIdx.x * 256u + threadIdx.x;
+    if (item >= items) return;
+    const int u = item % U, kv = p.c.kv_heads;
+    uint32_t hg, t;
+    const uint32_t bt = p.head_groups.div(item / U, hg), b = p.tokens.div(bt, t);
+    const long long start = p.start[(long long)b * p.start_stride], count = p.counts ? p.counts[b] : (long long)p.tokens.d;
+    const bool fits = kv4_fits(start, count, (int)p.tokens.d, p.c.max_len);
+    if (!fits) *p.status = 1;
+    uint32_t code[kKv4Heads];
+    float scale[kKv4Heads];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = s * ((float)(code >> (4 * j) & 15u) - 8.f);
+    for (int i = 0; i < kKv4Heads; ++i) {
+        const int h = (int)hg * kKv4Heads + i;
+        const bool key = h < kv;
+        code[i] = 0x88888888u, scale[i] = fits ? 0.f : __int_as_float(0x7fffffff);
+        if (h >= 2 * kv || !fits || t >= count) continue;
+        const size_t row = ((size_t)b * kv + (key ? h : h - kv)) * p.c.max_len + start + t;
+        code[i] = kv4_get_codes<D>((key ? p.c.k_codes : p.c.v_codes) + row * (D / 2), key, u);
+        scale[i] = __half2float((key ? p.c.k_scales : p.c.v_scales)[row * G + (u >> 2)]);
     }
-    *reinterpret_cast<uint2*>((is_k ? p.k_out : p.v_out) + (bt * kv + h) * D + lane * 4) = make_uint2(bf16_pack(x[0], x[1]), bf16_pack(x[2], x[3]));
+#pragma unroll
+    for (int i = 0; i < kKv4Heads; ++i) {
+        const int h = (int)hg * kKv4Heads + i;
+        if (h >= 2 * kv) continue;
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = scale[i] * ((float)(code[i] >> (4 * j) & 15u) - 8.f);
+        if (!(t < count)) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = fits ? 0.f : scale[i];
+        }
+        __nv_bfloat16* dst = h < kv ? p.k_out + ((long long)bt * kv + h) * D : p.v_out + ((long long)bt * kv + h - kv) * D;
+        *reinterpret_cast<uint4*>(dst + u * 8) = make_uint4(bf16_pack(x[0], x[1]), bf16_pack(x[2], x[3]), bf16_pack(x[4], x[5]), bf16_pack(x[6], x[7]));
+    }
 }
 
 }  // namespace tsp

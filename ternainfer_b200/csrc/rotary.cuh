@@ -10,6 +10,22 @@
 
 namespace tsp {
 
+// Division of 0 <= n < 2^31 by a number that the launch knows.
+struct FastDiv {
+    uint32_t d = 1, mul = 1, shift = 0;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t by) : d(by) {
+        while (shift < 31 && (1u << shift) < d) ++shift;
+        mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+    }
+    __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, mul) + n) >> shift; }
+    __device__ __forceinline__ uint32_t div(uint32_t n, uint32_t& rest) const {
+        const uint32_t q = div(n);
+        rest = n - q * d;
+        return q;
+    }
+};
+
 struct RotateSide {                        // queries or keys
     const void* x;
     void* y;                               // contiguous [B][T][heads][D]
@@ -22,8 +38,9 @@ struct RotateParams {
     const float *cos_tab, *sin_tab;        // [table_len][rotary / 2]
     const long long* pos;
     long long pos_sb, pos_st;
-    long long tokens_all;                  // batch * tokens
-    int tokens, dim, rotary, table_len;
+    FastDiv units, head_groups, tokens;
+    int dim, rotary, table_len;
+    int tables_16;                         // whether every table row starts on 16 bytes
     float sign;                            // of the sines
     int* status;
 };
@@ -48,52 +65,64 @@ template <> struct Elem<float> {
 template <typename T, int N>
 struct alignas(sizeof(T) * N) Vec { T v[N]; };
 
+// N consecutive values of a table row.
+template <int N>
+__device__ __forceinline__ void table_values(const float* t, int by_16, float (&x)[N]) {
+    if (N % 4 == 0 && by_16) {
+#pragma unroll
+        for (int i = 0; i + 3 < N; i += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(t + i);
+            x[i] = v.x, x[i + 1] = v.y, x[i + 2] = v.z, x[i + 3] = v.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = t[i];
+    }
+}
+
 // A thread takes one unit of a token - V pairs of the half layout, V / 2 of the other, or V copied values - in HEADS heads, so that
-// cosines and sines are read once for all of them.
+// cosines and sines are read once for all of them.  Memory is the bound: what matters is that all loads of a thread are on their way
+// before the first is used, and that the index arithmetic (divisions by multiplication, 32 bits) stays small beside them.
 template <typename T, int V, bool HALF, int HEADS>
-__global__ void __launch_bounds__(256) rotate_kernel(const RotateParams p, int units, int head_groups, long long items) {
+__global__ void __launch_bounds__(256, 4) rotate_kernel(const RotateParams p, uint32_t items) {
     using VT = Vec<T, V>;
-    const long long item = (long long)blockIdx.x * 256 + threadIdx.x;
+    const uint32_t item = blockIdx.x * 256u + threadIdx.x;
     if (item >= items) return;
-    const int u = (int)(item % units);
-    const long long r = item / units;
-    const int hg = (int)(r % head_groups);
-    const long long bt = r / head_groups, b = bt / p.tokens, t = bt - b * p.tokens;
+    uint32_t u, hg, t;
+    const uint32_t bt = p.head_groups.div(p.units.div(item, u), hg), b = p.tokens.div(bt, t);
     const int half = p.rotary / 2, turned = HALF ? half / V : p.rotary / V;
     constexpr int PAIRS = HALF ? V : (V > 1 ? V / 2 : 1);
-    const bool copies = u >= turned;
-    const int e = HALF && copies ? p.rotary + (u - turned) * V : u * V;   // first element
+    const bool copies = (int)u >= turned;
+    const int e = HALF && copies ? p.rotary + ((int)u - turned) * V : (int)u * V;   // first element
+    VT x[HEADS], y[HEADS];
+#pragma unroll
+    for (int i = 0; i < HEADS; ++i) {
+        const int h = (int)hg * HEADS + i, hk = h - p.q.heads;
+        const RotateSide& sd = hk < 0 ? p.q : p.k;
+        const int hh = hk < 0 ? h : hk;
+        if (hh >= sd.heads) continue;
+        const T* src = static_cast<const T*>(sd.x) + (long long)b * sd.sb + (long long)t * sd.st + (long long)hh * sd.sh + e;
+        x[i] = *reinterpret_cast<const VT*>(src);
+        if (HALF && !copies) y[i] = *reinterpret_cast<const VT*>(src + half);
+    }
     float c[PAIRS], s[PAIRS];
     if (!copies) {
         const long long pos = p.pos[b * p.pos_sb + t * p.pos_st];
         const bool ok = pos >= 0 && pos < p.table_len;
         const long long row = (ok ? pos : 0) * half + (HALF ? e : e / 2);
+        table_values(p.cos_tab + row, p.tables_16, c);
+        table_values(p.sin_tab + row, p.tables_16, s);
+        if (!ok) *p.status = 1;                                    // a position outside of the table
 #pragma unroll
-        for (int i = 0; i < PAIRS; ++i) c[i] = p.cos_tab[row + i], s[i] = p.sign * p.sin_tab[row + i];
-        if (!ok) {                                                 // a position outside of the table
-#pragma unroll
-            for (int i = 0; i < PAIRS; ++i) c[i] = s[i] = __int_as_float(0x7fffffff);
-            *p.status = 1;
-        }
-    }
-    VT x[HEADS], y[HEADS];
-    const T* src[HEADS];
-    T* dst[HEADS];
-#pragma unroll
-    for (int i = 0; i < HEADS; ++i) {
-        const int h = hg * HEADS + i;
-        const bool is_q = h < p.q.heads;
-        const RotateSide& sd = is_q ? p.q : p.k;
-        const int hh = is_q ? h : h - p.q.heads;
-        src[i] = hh < sd.heads ? static_cast<const T*>(sd.x) + b * sd.sb + t * sd.st + hh * sd.sh + e : nullptr;
-        dst[i] = static_cast<T*>(sd.y) + (bt * sd.heads + hh) * p.dim + e;
-        if (!src[i]) continue;
-        x[i] = *reinterpret_cast<const VT*>(src[i]);
-        if (HALF && !copies) y[i] = *reinterpret_cast<const VT*>(src[i] + half);
+        for (int i = 0; i < PAIRS; ++i) c[i] = ok ? c[i] : __int_as_float(0x7fffffff), s[i] *= p.sign;
     }
 #pragma unroll
     for (int i = 0; i < HEADS; ++i) {
-        if (!src[i]) continue;
+        const int h = (int)hg * HEADS + i, hk = h - p.q.heads;
+        const RotateSide& sd = hk < 0 ? p.q : p.k;
+        const int hh = hk < 0 ? h : hk;
+        if (hh >= sd.heads) continue;
+        T* dst = static_cast<T*>(sd.y) + ((long long)bt * sd.heads + hh) * p.dim + e;
         if (!copies) {
             if (HALF) {
 #pragma unroll
@@ -101,7 +130,7 @@ __global__ void __launch_bounds__(256) rotate_kernel(const RotateParams p, int u
                     const float a = Elem<T>::get(x[i].v[j]), bb = Elem<T>::get(y[i].v[j]);
                     x[i].v[j] = Elem<T>::put(rot_a(a, bb, c[j], s[j])), y[i].v[j] = Elem<T>::put(rot_b(a, bb, c[j], s[j]));
                 }
-                *reinterpret_cast<VT*>(dst[i] + half) = y[i];
+                *reinterpret_cast<VT*>(dst + half) = y[i];
             } else {
 #pragma unroll
                 for (int j = 0; j < V / 2; ++j) {
@@ -110,7 +139,7 @@ __global__ void __launch_bounds__(256) rotate_kernel(const RotateParams p, int u
                 }
             }
         }
-        *reinterpret_cast<VT*>(dst[i]) = x[i];
+        *reinterpret_cast<VT*>(dst) = x[i];
     }
 }
 
