@@ -24,6 +24,7 @@
 #include "dense_prefill.cuh"
 #include "kv4.cuh"
 #include "kv4_attn.cuh"
+#include "kv4_prefill.cuh"
 #include "lm_head.cuh"
 #include "logprobs.cuh"
 #include "mma_rate_probe.cuh"
@@ -1310,10 +1311,16 @@ extern "C" int ternaspmm_kv4_read(void* k_codes, void* k_scales, void* v_codes, 
 // each or, with `stream`, that many CTAs for everything.
 struct Kv4Plan {
     int tiles, row_tiles, cluster, stream;
+    bool tcgen05;                          // kv4_prefill_kernel, row_tiles of 128 rows
 };
-static Kv4Plan kv4_plan(int batch, int tokens, int heads, int kv_heads, int max_len) {
+static Kv4Plan kv4_plan(int batch, int tokens, int heads, int kv_heads, int max_len, int window) {
     const long long rows_all = (long long)tokens * (heads / kv_heads);
-    Kv4Plan pl = {rows_all <= 8 ? 1 : 2, 1, 1, 0};
+    Kv4Plan pl = {rows_all <= 8 ? 1 : 2, 1, 1, 0, false};
+    if (window == 0 && rows_all >= 128) {
+        pl.tcgen05 = true;
+        pl.row_tiles = (int)((rows_all + kKvpRows - 1) / kKvpRows);
+        return pl;
+    }
     pl.row_tiles = (int)((rows_all + 8 * pl.tiles - 1) / (8 * pl.tiles));
     const int slots = (pl.tiles == 1 ? 4 : 2) * device_sm_count();
     const long long items = (long long)batch * kv_heads * pl.row_tiles, blocks = max_len / 32;
@@ -1330,7 +1337,7 @@ static bool kv4_attend_shape(int batch, int tokens, int heads, int kv_heads, int
 
 extern "C" long long ternaspmm_kv4_attend_workspace(int batch, int tokens, int heads, int kv_heads, int head_dim, int max_len) {
     if (!kv4_attend_shape(batch, tokens, heads, kv_heads, head_dim, max_len)) return -1;
-    const Kv4Plan pl = kv4_plan(batch, tokens, heads, kv_heads, max_len);
+    const Kv4Plan pl = kv4_plan(batch, tokens, heads, kv_heads, max_len, 1);   // (a windowed call asks for the most)
     return (long long)pl.stream * 2 * 8 * pl.tiles * (head_dim + 2) * 4;
 }
 
@@ -1377,6 +1384,25 @@ static cudaError_t launch_kv4_attend(const Kv4AttnParams& p, int stream_ctas, cu
     return cudaLaunchKernelEx(&cfg, kv4_attn_join_kernel<D, NT>, p, stream_ctas, here);
 }
 
+template <int D>
+static cudaError_t launch_kv4_prefill(const Kv4AttnParams& p, cudaStream_t stream) {
+    static bool done[64] = {false};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) dev = 0;
+    if (!done[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(kv4_prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, KvpSmem<D>::total);
+        if (e != cudaSuccess) return e;
+        done[dev] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((long long)p.row_tiles * p.c.kv_heads), p.batch, 1);
+    cfg.blockDim = dim3(kKvpThreads, 1, 1);
+    cfg.dynamicSmemBytes = KvpSmem<D>::total;
+    cfg.stream = stream;
+    return cudaLaunchKernelEx(&cfg, kv4_prefill_kernel<D>, p);
+}
+
 extern "C" int ternaspmm_kv4_attend(const __nv_bfloat16* q, const long long* q_strides, void* k_codes, void* k_scales, void* v_codes, void* v_scales,
                                     int max_len, const long long* start, int start_stride, const long long* counts, int window, float scale,
                                     __nv_bfloat16* out, int batch, int tokens, int heads, int kv_heads, int head_dim, void* workspace,
@@ -1390,12 +1416,13 @@ extern "C" int ternaspmm_kv4_attend(const __nv_bfloat16* q, const long long* q_s
         (reinterpret_cast<uintptr_t>(out) & 15) || (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15))))
         return t_host_status = ST_BAD_POINTER;
     if (!p.status) return t_host_status = ST_LAUNCH;
-    const Kv4Plan pl = kv4_plan(batch, tokens, heads, kv_heads, max_len);
+    const Kv4Plan pl = kv4_plan(batch, tokens, heads, kv_heads, max_len, window);
     p.start = start, p.counts = counts, p.start_stride = start_stride ? 1 : 0, p.out = out, p.tokens = tokens, p.heads = heads, p.window = window;
     p.batch = batch, p.cluster = pl.cluster, p.row_tiles = pl.row_tiles, p.row_bytes = head_dim / 2, p.scale_log2 = scale * 1.4426950408889634f;
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = reinterpret_cast<float2*>(p.part_o + (size_t)pl.stream * 2 * 8 * pl.tiles * head_dim);
-    const cudaError_t e = head_dim == 128 ? (pl.tiles == 1 ? launch_kv4_attend<128, 1>(p, pl.stream, stream) : launch_kv4_attend<128, 2>(p, pl.stream, stream))
+    const cudaError_t e = pl.tcgen05 ? (head_dim == 128 ? launch_kv4_prefill<128>(p, stream) : launch_kv4_prefill<64>(p, stream))
+                          : head_dim == 128 ? (pl.tiles == 1 ? launch_kv4_attend<128, 1>(p, pl.stream, stream) : launch_kv4_attend<128, 2>(p, pl.stream, stream))
                                           : (pl.tiles == 1 ? launch_kv4_attend<64, 1>(p, pl.stream, stream) : launch_kv4_attend<64, 2>(p, pl.stream, stream));
     if (e != cudaSuccess) t_host_status = ST_LAUNCH;
     checkLastCudaError(__LINE__);

@@ -59,6 +59,11 @@ def attention(q, k, v, start, counts, window, scale):
     q_size = (q.double().abs().amax(-1) * q.shape[-1]).permute(0, 2, 1) * kk.abs().amax((1, 3))[:, :, None] * scale
     lost = size * (2.0 ** -10 + 2.0 ** -13) + top * (n * 2.0 ** -24 * 2 + (n / 16 + 1) * 2.0 ** -21) + \
         (q_size * 2.0 ** -20).permute(0, 2, 1)[..., None] * size
+    if T > 1:
+        # Calls of many tokens round keys and values to fp16: 2^-11 of every product |q||k|, an exponent of the probability and of their sum, and
+        # 2^-11 of every value.
+        s_abs = (torch.einsum("bthd,blhd->bhtl", q.double().abs(), kk.abs()) * scale).masked_fill(~sees[:, None], 0).amax(-1)
+        lost = lost + size * (2.0 ** -11 + 2.0 ** -10 * s_abs.permute(0, 2, 1)[..., None])
     # What is rounded to bf16 is the result with those errors: |r(out + e) - out| <= |e| + 2^-8 |out + e| <= lost + 2^-8 (|out| + lost)
     return out, lost + (out.abs() + lost) * 2.0 ** -8
 
@@ -147,7 +152,7 @@ def test_attend_one_token(lib, D, H, K, B, past, L):
 
 
 @pytest.mark.parametrize("D,H,K", [(128, 20, 5), (64, 8, 8), (128, 6, 2), (128, 17, 1)])
-@pytest.mark.parametrize("B,T,past", [(1, 2, 0), (2, 5, 11), (1, 17, 0), (1, 64, 64), (2, 100, 77), (1, 333, 200)])
+@pytest.mark.parametrize("B,T,past", [(1, 2, 0), (2, 5, 11), (1, 17, 0), (1, 64, 64), (2, 100, 77), (1, 333, 200), (1, 128, 0), (3, 129, 1000), (2, 700, 63)])
 def test_attend_several_tokens(lib, D, H, K, B, T, past):
     cache, k, v = filled(B, K, past + T + 20, D, past + T, spread=2.0)
     qkv = torch.randn((B, T, H + 2 * K, D), generator=gen(T), device="cuda").to(torch.bfloat16)
@@ -242,6 +247,21 @@ def test_what_is_not_seen_does_not_matter(lib, T):
     cache.v_scales[0, 1, 0, 2] = float("nan")                      # one group of one key, seen by all
     out = kv4_attend(q, cache, start)
     assert out[0, :, 4:, 64:96].isnan().all() and out[0, :-1, 4:, :64].isfinite().all() and out[0, :-1, :4].isfinite().all()
+
+
+def test_values_beyond_fp16_among_many_tokens(lib):
+    """Scales that make values beyond 65504: the rows that see one have NaN in its group, the others their results."""
+    B, T, H, K, D = 1, 200, 4, 1, 128
+    cache, k, v = filled(B, K, T, D, 3)
+    q = torch.randn((B, T, H, D), generator=gen(4), device="cuda").to(torch.bfloat16)
+    start = torch.zeros(1, dtype=torch.int64, device="cuda")
+    want = check(q, cache, k, v, start)
+    cache.v_scales[0, 0, 70, 1], cache.v_scales[0, 0, 150, 3] = 60000.0, float("-inf")
+    out = kv4_attend(q, cache, start)
+    lost = torch.zeros((T, D), dtype=torch.bool, device="cuda")
+    lost[70:, 32:64], lost[150:, 96:] = True, True
+    assert torch.equal(out.isnan(), lost[None, :, None].expand_as(out)) and torch.equal(out[0][:, :, :32], want[0][:, :, :32])
+    assert torch.equal(out[0].masked_fill(lost[:, None], 0), want[0].masked_fill(lost[:, None], 0))
 
 
 def test_infinite_and_nan_inputs_stay_in_their_group(lib):
