@@ -77,6 +77,28 @@ __device__ __forceinline__ uint32_t kvp_high(uint32_t x, uint32_t scales) {
     return f16x2_mul(f16x2_fma((x & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd480d480u), scales);   // / 16 - 72
 }
 
+template <int WORDS>
+__device__ __forceinline__ void ldg_words(const void* src, uint32_t (&w)[WORDS]) {
+    if constexpr (WORDS == 2) {
+        const uint2 v = *static_cast<const uint2*>(src);
+        w[0] = v.x, w[1] = v.y;
+    } else {
+        w[0] = *static_cast<const uint32_t*>(src);
+    }
+}
+// One arrival for a warp, after all of its lanes' writes (64 and 128 arrivals of single threads on one barrier took as long as a product).
+__device__ __forceinline__ void kvp_arrive(uint32_t bar, int lane) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+}
+__device__ __forceinline__ bool kvp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+#pragma unroll 1
+    for (int i = 0; i < 256; ++i)
+        if (mbar_test(bar, parity)) return true;
+    return wait_longer(bar, parity, abort_flag);
+}
+__device__ __forceinline__ bool kvp_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag) { return __all_sync(0xffffffffu, kvp_wait(bar, parity, abort_flag)); }
+
 template <int D>
 __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4AttnParams p) {
     using Sm = KvpSmem<D>;
@@ -95,11 +117,11 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
     const Kv4Range rg = kv4_range(p.start, p.counts, p.start_stride, b, p.tokens, 0, p.c.max_len, t_first, r_last / per_kv);
     const int tiles = (rg.hi + kKvpKeys - 1) / kKvpKeys;
     if (tid == 0) {
-        mbar_init(b_q, kKvpRows);
+        mbar_init(b_q, 4);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(b_kf + 8 * i, 64), mbar_init(b_ke + 8 * i, 1);
-            mbar_init(b_vf + 8 * i, 64), mbar_init(b_ve + 8 * i, 1);
-            mbar_init(b_s + 8 * i, 1), mbar_init(b_p + 8 * i, kKvpRows);
+            mbar_init(b_kf + 8 * i, 2), mbar_init(b_ke + 8 * i, 1);
+            mbar_init(b_vf + 8 * i, 2), mbar_init(b_ve + 8 * i, 1);
+            mbar_init(b_s + 8 * i, 1), mbar_init(b_p + 8 * i, 4);
         }
         mbar_init(b_o, 1);
         mbar_fence_init();
@@ -146,12 +168,12 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
             }
         }
         fence_proxy_async_smem();
-        mbar_arrive(b_q);
+        kvp_arrive(b_q, lane);
         float top = -INFINITY, nb = 0.f;                           // as in kv4_attn_kernel
 #pragma unroll 1
         for (int j = 0; j < tiles; ++j) {
             const int buf = j & 1;
-            ok = wait_warp(b_s + 8 * buf, (j >> 1) & 1, abort_flag);
+            ok = kvp_wait_warp(b_s + 8 * buf, (j >> 1) & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
             const uint32_t ts = t_s + mine + buf * 64;
@@ -167,9 +189,10 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
                 for (int i = 0; i < 64; ++i)
                     if (i > sees) s[i >> 5][i & 31] = -INFINITY;
             }
-            float mx = s[0][0];
+            float m4[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};   // (four chains: one would take as long as the exponentials)
 #pragma unroll
-            for (int i = 1; i < 64; ++i) mx = fmaxf(mx, s[i >> 5][i & 31]);
+            for (int i = 4; i < 64; ++i) m4[i & 3] = fmaxf(m4[i & 3], s[i >> 5][i & 31]);
+            const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
             const bool grown = mx > top;
             if (__any_sync(0xffffffffu, grown)) {
                 float f = 1.f;
@@ -180,7 +203,7 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
                 }
                 l *= f;
                 if (j > 0) {                                       // O is complete up to tile j - 1 before it is touched
-                    ok = wait_warp(b_o, (j - 1) & 1, abort_flag);
+                    ok = kvp_wait_warp(b_o, (j - 1) & 1, abort_flag);
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll 1
@@ -199,40 +222,46 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
                     tmem_st_wait();
                 }
             }
+            float l2[2] = {0.f, 0.f};
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 uint32_t w[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const float x = ex2_approx(fmaf(s[half][2 * i], row_f, nb)), y = ex2_approx(fmaf(s[half][2 * i + 1], row_f, nb));
-                    l += x + y;
+                    l2[i & 1] += x + y;
                     w[i] = f16_pack(x, y);
                 }
                 tmem_st16(ts + 16 * half, w);
             }
+            l += l2[0] + l2[1];
             tmem_st_wait();
             tc_fence_before();
-            mbar_arrive(b_p + 8 * buf);
+            kvp_arrive(b_p + 8 * buf, lane);
         }
-        if (ok && tiles > 0) ok = wait_warp(b_o, (tiles - 1) & 1, abort_flag);
+        if (ok && tiles > 0) ok = kvp_wait_warp(b_o, (tiles - 1) & 1, abort_flag);
     } else if (warp < 6) {                                         // ---- keys: one per thread
         const int key = tid - 128;
         const uint8_t* kc = p.c.k_codes + (row0 + key) * (D / 2);
         const __half* ks = p.c.k_scales + (row0 + key) * G;
-        uint4 w[D / 32];
-        uint32_t sc[G / 2];
-        auto load = [&](int j) {
+        uint4 w[D / 32], w_next[D / 32];                           // (the next tile is on its way while one is expanded)
+        uint32_t sc[G / 2], sc_next[G / 2];
+        auto load = [&](int j, uint4 (&w)[D / 32], uint32_t (&sc)[G / 2]) {
             const uint8_t* src = kc + (size_t)j * kKvpKeys * (D / 2);
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) w[i] = ldg_128(src + 16 * i);
-#pragma unroll
-            for (int i = 0; i < G / 2; ++i) sc[i] = reinterpret_cast<const uint32_t*>(ks + (size_t)j * kKvpKeys * G)[i];
+            ldg_words(ks + (size_t)j * kKvpKeys * G, sc);
         };
-        if (tiles > 0) load(0);
+        if (tiles > 0) load(0, w_next, sc_next);
 #pragma unroll 1
         for (int j = 0; j < tiles; ++j) {
             const int st = j & 1;
-            if (j >= 2 && !wait_warp(b_ke + 8 * st, ((j >> 1) - 1) & 1, abort_flag)) break;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) w[i] = w_next[i];
+#pragma unroll
+            for (int i = 0; i < G / 2; ++i) sc[i] = sc_next[i];
+            if (j + 1 < tiles) load(j + 1, w_next, sc_next);
+            if (j >= 2 && !kvp_wait_warp(b_ke + 8 * st, ((j >> 1) - 1) & 1, abort_flag)) break;
             const uint32_t dst = sb + Sm::k + st * Sm::k_bytes + key * 128;
             // 16 bytes t of a row hold word t of every group (64 dimensions: 8 bytes)
             uint32_t words[4 * G];
@@ -248,42 +277,48 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
                     sts128(dst + (c >> 3) * Sm::k_block + (((c & 7) ^ (key & 7)) << 4), make_uint4(kvp_low(x, f), kvp_high(x, f), kvp_low(x8, f), kvp_high(x8, f)));
                 }
             }
-            if (j + 1 < tiles) load(j + 1);
             fence_proxy_async_smem();
-            mbar_arrive(b_kf + 8 * st);
+            kvp_arrive(b_kf + 8 * st, lane);
         }
     } else if (warp < 8) {                                         // ---- values: 16 dimensions of 8 keys per thread
         const int oct = tid & 7, g = (tid - 192) >> 3;             // keys 8 oct .. + 7, halfword g of every group
         const uint8_t* vc = p.c.v_codes + (row0 + 8 * oct) * (D / 2) + g * (G * 2);
         const __half* vs = p.c.v_scales + (row0 + 8 * oct) * G;
-        uint32_t w[8][G / 2], sc[8][G / 2];
-        auto load = [&](int j) {
+        uint32_t w[8][G / 2], sc[8][G / 2], w_next[8][G / 2], sc_next[8][G / 2];
+        auto load = [&](int j, uint32_t (&w)[8][G / 2], uint32_t (&sc)[8][G / 2]) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const uint8_t* src = vc + ((size_t)j * kKvpKeys + k) * (D / 2);
-                const __half* s = vs + ((size_t)j * kKvpKeys + k) * G;
-#pragma unroll
-                for (int i = 0; i < G / 2; ++i) w[k][i] = reinterpret_cast<const uint32_t*>(src)[i], sc[k][i] = reinterpret_cast<const uint32_t*>(s)[i];
+                ldg_words(vc + ((size_t)j * kKvpKeys + k) * (D / 2), w[k]);
+                ldg_words(vs + ((size_t)j * kKvpKeys + k) * G, sc[k]);
             }
         };
-        if (tiles > 0) load(0);
+        if (tiles > 0) load(0, w_next, sc_next);
 #pragma unroll 1
         for (int j = 0; j < tiles; ++j) {
             const int st = j & 1, key0 = j * kKvpKeys + 8 * oct;
-            if (j >= 2 && !wait_warp(b_ve + 8 * st, ((j >> 1) - 1) & 1, abort_flag)) break;
-            const uint32_t dst = sb + Sm::v + st * Sm::v_bytes;
-            // keys behind the last one hold anything; scales beyond 8188 (0x6fff) make values that fp16 does not hold
 #pragma unroll
             for (int k = 0; k < 8; ++k)
 #pragma unroll
-                for (int i = 0; i < G / 2; ++i) {
-                    if (key0 + k >= rg.hi) sc[k][i] = 0u;
-                    const uint32_t lo = sc[k][i] & 0x7fffu, hi = sc[k][i] >> 16 & 0x7fffu;
-                    if (lo > 0x6fffu || hi > 0x6fffu) {
-                        if (lo > 0x6fffu) atomicMin(&bad[2 * i], key0 + k), sc[k][i] &= 0xffff0000u;
-                        if (hi > 0x6fffu) atomicMin(&bad[2 * i + 1], key0 + k), sc[k][i] &= 0x0000ffffu;
+                for (int i = 0; i < G / 2; ++i) w[k][i] = w_next[k][i], sc[k][i] = sc_next[k][i];
+            if (j + 1 < tiles) load(j + 1, w_next, sc_next);
+            if (j >= 2 && !kvp_wait_warp(b_ve + 8 * st, ((j >> 1) - 1) & 1, abort_flag)) break;
+            const uint32_t dst = sb + Sm::v + st * Sm::v_bytes;
+            // keys behind the last one hold anything; scales beyond 8188 (0x6fff) make values that fp16 does not hold
+            uint32_t big = 0;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+#pragma unroll
+                for (int i = 0; i < G / 2; ++i) big = __vmaxu2(big, sc[k][i] & 0x7fff7fffu);
+            if ((j + 1) * kKvpKeys > rg.hi || __vcmpgtu2(big, 0x6fff6fffu)) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+#pragma unroll
+                    for (int i = 0; i < G / 2; ++i) {
+                        if (key0 + k >= rg.hi) sc[k][i] = 0u;
+                        if ((sc[k][i] & 0x7fffu) > 0x6fffu) atomicMin(&bad[2 * i], key0 + k), sc[k][i] &= 0xffff0000u;
+                        if ((sc[k][i] >> 16 & 0x7fffu) > 0x6fffu) atomicMin(&bad[2 * i + 1], key0 + k), sc[k][i] &= 0x0000ffffu;
                     }
-                }
+            }
 #pragma unroll
             for (int i = 0; i < G; ++i) {
                 const uint32_t sel = i & 1 ? 0x7632 : 0x5410;
@@ -299,17 +334,16 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
                     sts128(dst + d * 128 + ((oct ^ (d & 7)) << 4), make_uint4(out[n][0], out[n][1], out[n][2], out[n][3]));
                 }
             }
-            if (j + 1 < tiles) load(j + 1);
             fence_proxy_async_smem();
-            mbar_arrive(b_vf + 8 * st);
+            kvp_arrive(b_vf + 8 * st, lane);
         }
     } else if (lane == 0) {                                        // ---- products
         const uint32_t id_s = (1u << 4) | ((uint32_t)(kKvpKeys >> 3) << 17) | ((uint32_t)(kKvpRows >> 4) << 24);
         const uint32_t id_o = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kKvpRows >> 4) << 24);
-        ok = tiles == 0 || wait_suspended(b_q, 0, abort_flag);
+        ok = tiles == 0 || kvp_wait(b_q, 0, abort_flag);
         auto scores = [&](int j) {
             const int st = j & 1;
-            if (!wait_suspended(b_kf + 8 * st, (j >> 1) & 1, abort_flag)) return false;
+            if (!kvp_wait(b_kf + 8 * st, (j >> 1) & 1, abort_flag)) return false;
             tc_fence_after();
             const uint32_t k = sb + Sm::k + st * Sm::k_bytes;
 #pragma unroll
@@ -324,8 +358,8 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
         for (int j = 0; ok && j < tiles; ++j) {
             const int st = j & 1;
             // the buffer that the scores of tile j + 1 go to is the one that the product of tile j - 1 with V reads
-            if (j + 1 < tiles) ok = (j == 0 || wait_suspended(b_o, (j - 1) & 1, abort_flag)) && scores(j + 1);
-            ok = ok && wait_suspended(b_vf + 8 * st, (j >> 1) & 1, abort_flag) && wait_suspended(b_p + 8 * st, (j >> 1) & 1, abort_flag);
+            if (j + 1 < tiles) ok = (j == 0 || kvp_wait(b_o, (j - 1) & 1, abort_flag)) && scores(j + 1);
+            ok = ok && kvp_wait(b_vf + 8 * st, (j >> 1) & 1, abort_flag) && kvp_wait(b_p + 8 * st, (j >> 1) & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
             const uint32_t v = sb + Sm::v + st * Sm::v_bytes;
