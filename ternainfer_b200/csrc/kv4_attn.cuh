@@ -24,10 +24,10 @@ struct Kv4AttnParams {
     const long long *start, *counts;
     int start_stride;
     __nv_bfloat16* out;                    // [B][T][heads][D]
-    float* part_o;                         // KV4_STREAM: [CTA][first, last item][rows][D]
-    float2* part_ml;                       // [CTA][first, last item][rows]: reference of the exponents, sum
+    float* part_o;                         // KV4_STREAM: [CTA][first, last item][rows][D]; kv4_prefill_kernel in parts: [CTA][rows][D]
+    float2* part_ml;                       // the same without [D]: reference of the exponents, sum
     int batch, tokens, heads, window;
-    int cluster, row_tiles, row_bytes;     // CTAs of a cluster; tiles of rows per key / value head; bytes of a row's codes, D / 2
+    int cluster, row_tiles, row_bytes;     // CTAs of a cluster (kv4_prefill_kernel: for a tile); tiles of rows per key / value head; D / 2
     float scale_log2;                      // log2(e) * softmax scale
     int* status;
 };

@@ -111,11 +111,13 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Sm::abort_flag);
     int* bad = reinterpret_cast<int*>(smem + Sm::bad);
     // the longest rows first
-    const int tile = p.row_tiles - 1 - blockIdx.x / p.c.kv_heads, hk = blockIdx.x % p.c.kv_heads, b = blockIdx.y;
+    const int part = blockIdx.x % p.cluster, item = blockIdx.x / p.cluster, tile = p.row_tiles - 1 - item / p.c.kv_heads, hk = item % p.c.kv_heads, b = blockIdx.y;
     const int per_kv = p.heads / p.c.kv_heads, rows_all = p.tokens * per_kv, r0 = tile * kKvpRows, r_last = min(r0 + kKvpRows, rows_all) - 1;
     const int t_first = r0 / per_kv;
-    const Kv4Range rg = kv4_range(p.start, p.counts, p.start_stride, b, p.tokens, 0, p.c.max_len, t_first, r_last / per_kv);
-    const int tiles = (rg.hi + kKvpKeys - 1) / kKvpKeys;
+    const Kv4Range rg = kv4_range(p.start, p.counts, p.start_stride, b, p.tokens, p.window, p.c.max_len, t_first, r_last / per_kv);
+    // key tiles of this CTA: its part of those that some row sees; `base`, the first
+    const int j_lo = rg.lo / kKvpKeys, j_all = (rg.hi + kKvpKeys - 1) / kKvpKeys - j_lo;
+    const int j0 = (int)((long long)j_all * part / p.cluster), tiles = (int)((long long)j_all * (part + 1) / p.cluster) - j0, base = (j_lo + j0) * kKvpKeys;
     if (tid == 0) {
         mbar_init(b_q, 4);
         for (int i = 0; i < 2; ++i) {
@@ -134,12 +136,12 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + Sm::slot), t_o = tmem, t_s = tmem + 128;
-    const size_t row0 = ((size_t)b * p.c.kv_heads + hk) * p.c.max_len;
+    const size_t row0 = ((size_t)b * p.c.kv_heads + hk) * p.c.max_len + base;
     // warps 0 .. 3: this thread's row, its sum and whether all went well
     const int row = r0 + min(tid, kKvpRows - 1), t = min(row, rows_all - 1) / per_kv, h = hk * per_kv + min(row, rows_all - 1) % per_kv;
-    const int pos = rg.first_pos - t_first + t;
+    const int pos = rg.first_pos - t_first + t, seen_from = p.window ? max(pos - p.window + 1, 0) : 0, seen_to = min(pos, rg.limit - 1);
     const uint32_t mine = (uint32_t)(warp * 32) << 16;
-    float l = 0.f;
+    float l = 0.f, nb = 0.f;                                       // sum, minus the reference of the exponents
     bool ok = true;
 
     if (warp < 4) {
@@ -169,7 +171,7 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
         }
         fence_proxy_async_smem();
         kvp_arrive(b_q, lane);
-        float top = -INFINITY, nb = 0.f;                           // as in kv4_attn_kernel
+        float top = -INFINITY;                                     // as in kv4_attn_kernel
 #pragma unroll 1
         for (int j = 0; j < tiles; ++j) {
             const int buf = j & 1;
@@ -182,12 +184,18 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
             tmem_ld32(ts + 32, s[1]);
             tmem_ld32_wait(s[0]);
             tmem_ld32_wait(s[1]);
-            const int key0 = j * kKvpKeys;
+            const int key0 = base + j * kKvpKeys;
             if (key0 + kKvpKeys - 1 > rg.first_pos || key0 + kKvpKeys > rg.limit) {
-                const int sees = min(pos, rg.limit - 1) - key0;    // the last key of the tile that the row sees
+                const int sees = seen_to - key0;                   // the last key of the tile that the row sees
 #pragma unroll
                 for (int i = 0; i < 64; ++i)
                     if (i > sees) s[i >> 5][i & 31] = -INFINITY;
+            }
+            if (__any_sync(0xffffffffu, seen_from > key0)) {
+                const int from = seen_from - key0;                 // the first one
+#pragma unroll
+                for (int i = 0; i < 64; ++i)
+                    if (i < from) s[i >> 5][i & 31] = -INFINITY;
             }
             float m4[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};   // (four chains: one would take as long as the exponentials)
 #pragma unroll
@@ -295,7 +303,7 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
         if (tiles > 0) load(0, w_next, sc_next);
 #pragma unroll 1
         for (int j = 0; j < tiles; ++j) {
-            const int st = j & 1, key0 = j * kKvpKeys + 8 * oct;
+            const int st = j & 1, key0 = base + j * kKvpKeys + 8 * oct;
 #pragma unroll
             for (int k = 0; k < 8; ++k)
 #pragma unroll
@@ -309,7 +317,7 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
             for (int k = 0; k < 8; ++k)
 #pragma unroll
                 for (int i = 0; i < G / 2; ++i) big = __vmaxu2(big, sc[k][i] & 0x7fff7fffu);
-            if ((j + 1) * kKvpKeys > rg.hi || __vcmpgtu2(big, 0x6fff6fffu)) {
+            if (base + (j + 1) * kKvpKeys > rg.hi || __vcmpgtu2(big, 0x6fff6fffu)) {
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
 #pragma unroll
@@ -373,8 +381,12 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
     __syncthreads();                                               // (`bad` is complete)
     if (warp < 4) {
         tc_fence_after();
-        const float nan = __int_as_float(0x7fffffff), inv = l == 0.f ? 0.f : 1.f / l;
+        const float nan = __int_as_float(0x7fffffff);
+        const bool whole = p.cluster == 1;
+        const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
+        const size_t at = ((size_t)b * gridDim.x + blockIdx.x) * kKvpRows + tid;
         __nv_bfloat16* dst = p.out + (((size_t)b * p.tokens + t) * p.heads + h) * D;
+        if (!whole) p.part_ml[at] = make_float2(-nb, ok ? l : nan);
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
             float o[32];
@@ -382,10 +394,19 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
                 tmem_ld32(t_o + mine + c, o);
                 tmem_ld32_wait(o);
             }
-            const bool lost = !ok || !rg.ok || pos >= bad[c / 32];
+            bool lost = !ok || !rg.ok || seen_to >= bad[c / 32];
+            if (p.window && ok && rg.ok && lost) {                 // (`bad` is the first such key: is there one that this row sees?)
+                lost = false;
+                const __half* vs = p.c.v_scales + (row0 - base) * G + c / 32;
+                for (int key = max(seen_from, base); key <= min(seen_to, base + tiles * kKvpKeys - 1); ++key)
+                    lost |= (__half_as_ushort(vs[(size_t)key * G]) & 0x7fff) > 0x6fff;
+            }
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = lost ? nan : l == 0.f ? 0.f : o[i] * inv;
-            if (row < rows_all) {
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(p.part_o + at * D + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            } else if (row < rows_all) {
 #pragma unroll
                 for (int i = 0; i < 32; i += 8)
                     stg_128(dst + c + i, make_uint4(bf16_pack(o[i], o[i + 1]), bf16_pack(o[i + 2], o[i + 3]), bf16_pack(o[i + 4], o[i + 5]), bf16_pack(o[i + 6], o[i + 7])));
@@ -399,6 +420,43 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
         tc_fence_after();
         tmem_dealloc(tmem, Sm::columns);
     }
+}
+
+// Joins the parts of a row, a warp per row.  One that saw no key has sum 0 and stays out; NaN of a part's values or sum goes to the row.
+constexpr int kKvpJoinWarps = 8;
+template <int D>
+__global__ void __launch_bounds__(kKvpJoinWarps * 32) kv4_prefill_join_kernel(const Kv4AttnParams p) {
+    constexpr int DEEP = 8;                                        // parts on their way at once
+    const int lane = threadIdx.x & 31, per_kv = p.heads / p.c.kv_heads, rows = p.tokens * per_kv, b = blockIdx.y;
+    const long long at = (long long)blockIdx.x * kKvpJoinWarps + (threadIdx.x >> 5);
+    griddep_wait();
+    if (at >= (long long)rows * p.c.kv_heads) return;
+    const int hk = (int)(at / rows), row = (int)(at % rows);
+    const int item = (p.row_tiles - 1 - row / kKvpRows) * p.c.kv_heads + hk;
+    const size_t first = ((size_t)b * p.row_tiles * p.c.kv_heads + item) * p.cluster * kKvpRows + row % kKvpRows;
+    float top = -INFINITY, sum = 0.f;
+    float4 val = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = 0; c < p.cluster; c += DEEP) {
+        float2 ml[DEEP];
+        float4 y[DEEP];
+#pragma unroll
+        for (int j = 0; j < DEEP; ++j) {
+            ml[j] = make_float2(0.f, 0.f);
+            if (c + j >= p.cluster) continue;
+            const size_t from = first + (size_t)(c + j) * kKvpRows;
+            ml[j] = p.part_ml[from];
+            if (lane < D / 4) y[j] = *reinterpret_cast<const float4*>(p.part_o + from * D + lane * 4);
+        }
+#pragma unroll
+        for (int j = 0; j < DEEP; ++j) {
+            if (ml[j].y == 0.f) continue;
+            const float to = fmaxf(top, ml[j].x), f = top == -INFINITY ? 0.f : ex2_approx(top - to), g = ex2_approx(ml[j].x - to);
+            top = to, sum = sum * f + ml[j].y * g;
+            val.x = val.x * f + y[j].x * g, val.y = val.y * f + y[j].y * g, val.z = val.z * f + y[j].z * g, val.w = val.w * f + y[j].w * g;
+        }
+    }
+    const bool ok = kv4_range(p.start, p.counts, p.start_stride, b, p.tokens, p.window, p.c.max_len, 0, 0).ok;
+    if (lane < D / 4) kv4_store(p, ok, b, hk, per_kv, row, lane * 4, val, sum);
 }
 
 }  // namespace tsp

@@ -1311,19 +1311,27 @@ extern "C" int ternaspmm_kv4_read(void* k_codes, void* k_scales, void* v_codes, 
 // each or, with `stream`, that many CTAs for everything.
 struct Kv4Plan {
     int tiles, row_tiles, cluster, stream;
-    bool tcgen05;                          // kv4_prefill_kernel, row_tiles of 128 rows
+    bool tcgen05;                          // kv4_prefill_kernel, row_tiles of 128 rows, `cluster` CTAs for each
 };
-static Kv4Plan kv4_plan(int batch, int tokens, int heads, int kv_heads, int max_len, int window) {
+static Kv4Plan kv4_plan(int batch, int tokens, int heads, int kv_heads, int max_len) {
     const long long rows_all = (long long)tokens * (heads / kv_heads);
     Kv4Plan pl = {rows_all <= 8 ? 1 : 2, 1, 1, 0, false};
-    if (window == 0 && rows_all >= 128) {
+    pl.row_tiles = (int)((rows_all + 8 * pl.tiles - 1) / (8 * pl.tiles));
+    const int sms = device_sm_count(), slots = (pl.tiles == 1 ? 4 : 2) * sms;
+    const long long items = (long long)batch * kv_heads * pl.row_tiles, blocks = max_len / 32;
+    // Several tokens.  The mma.sync kernel goes over the keys once per 16 rows, with a cluster of up to 8 CTAs for each, and the tcgen05 kernel
+    // once per 128, in parts.  Up to SMs / 4 tiles of 16 rows the clusters are all resident: 12 tokens of 20 heads over 5, 3,000 keys, 10.8 against 17.5 us
+    // (24 tokens: 13.0 against 17.8; 32 tokens, 40 tiles: 8,000 keys, 36 against 21; 128 tokens: 84 against 38).  Below 2 SMs blocks of 32 keys
+    // in all there is too little to do: 64 tokens after none, 7.2 against 10.4 us.  One token stays with the mma.sync kernel, which takes values of any size.
+    if (tokens > 1 && pl.row_tiles > 1 && 4 * items > sms && items * blocks >= 2 * sms) {
         pl.tcgen05 = true;
         pl.row_tiles = (int)((rows_all + kKvpRows - 1) / kKvpRows);
+        // Parts of at least 4 tiles of 64 keys, a CTA per SM; two per SM take 1.5 times as long for a tile, so only where a part is longer than 16 tiles:
+        // 512 rows of 5 heads, 3,000 keys, 22.7 us with 7 parts and 28.5 with 12; 8 sequences of 128 rows, 30,000 keys, 152 us with 7 and 210 with 3.
+        const long long ctas = (long long)batch * kv_heads * pl.row_tiles, tiles = max_len / kKvpKeys, parts = sms / ctas;
+        pl.cluster = (int)std::max(1ll, std::min({tiles > 16 * parts ? 2 * sms / ctas : parts, tiles / 4, 32ll}));
         return pl;
     }
-    pl.row_tiles = (int)((rows_all + 8 * pl.tiles - 1) / (8 * pl.tiles));
-    const int slots = (pl.tiles == 1 ? 4 : 2) * device_sm_count();
-    const long long items = (long long)batch * kv_heads * pl.row_tiles, blocks = max_len / 32;
     if (pl.row_tiles == 1 && items * blocks >= 4ll * kKv4Warps * slots) {
         pl.stream = slots;
         return pl;
@@ -1331,14 +1339,18 @@ static Kv4Plan kv4_plan(int batch, int tokens, int heads, int kv_heads, int max_
     while (pl.cluster < 8 && pl.cluster * kKv4Warps < blocks && items * pl.cluster < 2 * slots) pl.cluster *= 2;
     return pl;
 }
+// Rows of partial results that a call keeps in its workspace.
+static long long kv4_part_rows(int batch, int kv_heads, const Kv4Plan& pl) {
+    if (!pl.tcgen05) return (long long)pl.stream * 2 * 8 * pl.tiles;
+    return pl.cluster > 1 ? (long long)batch * kv_heads * pl.row_tiles * pl.cluster * kKvpRows : 0;
+}
 static bool kv4_attend_shape(int batch, int tokens, int heads, int kv_heads, int head_dim, int max_len) {
     return kv4_shape(batch, tokens, kv_heads, head_dim, max_len) && heads >= kv_heads && heads % kv_heads == 0 && (long long)tokens * heads < (1ll << 30);
 }
 
 extern "C" long long ternaspmm_kv4_attend_workspace(int batch, int tokens, int heads, int kv_heads, int head_dim, int max_len) {
     if (!kv4_attend_shape(batch, tokens, heads, kv_heads, head_dim, max_len)) return -1;
-    const Kv4Plan pl = kv4_plan(batch, tokens, heads, kv_heads, max_len, 1);   // (a windowed call asks for the most)
-    return (long long)pl.stream * 2 * 8 * pl.tiles * (head_dim + 2) * 4;
+    return kv4_part_rows(batch, kv_heads, kv4_plan(batch, tokens, heads, kv_heads, max_len)) * (head_dim + 2) * 4;
 }
 
 template <int D, int NT>
@@ -1396,11 +1408,22 @@ static cudaError_t launch_kv4_prefill(const Kv4AttnParams& p, cudaStream_t strea
         done[dev] = true;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((long long)p.row_tiles * p.c.kv_heads), p.batch, 1);
+    cfg.gridDim = dim3((unsigned)((long long)p.row_tiles * p.c.kv_heads * p.cluster), p.batch, 1);
     cfg.blockDim = dim3(kKvpThreads, 1, 1);
     cfg.dynamicSmemBytes = KvpSmem<D>::total;
     cfg.stream = stream;
-    return cudaLaunchKernelEx(&cfg, kv4_prefill_kernel<D>, p);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kv4_prefill_kernel<D>, p);
+    if (e != cudaSuccess || p.cluster == 1) return e;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = tuning().pdl ? 1 : 0;
+    const long long rows = (long long)p.tokens * p.heads;
+    cfg.gridDim = dim3((unsigned)((rows + kKvpJoinWarps - 1) / kKvpJoinWarps), p.batch, 1);
+    cfg.blockDim = dim3(kKvpJoinWarps * 32, 1, 1);
+    cfg.dynamicSmemBytes = 0;
+    return cudaLaunchKernelEx(&cfg, kv4_prefill_join_kernel<D>, p);
 }
 
 extern "C" int ternaspmm_kv4_attend(const __nv_bfloat16* q, const long long* q_strides, void* k_codes, void* k_scales, void* v_codes, void* v_scales,
@@ -1416,11 +1439,11 @@ extern "C" int ternaspmm_kv4_attend(const __nv_bfloat16* q, const long long* q_s
         (reinterpret_cast<uintptr_t>(out) & 15) || (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15))))
         return t_host_status = ST_BAD_POINTER;
     if (!p.status) return t_host_status = ST_LAUNCH;
-    const Kv4Plan pl = kv4_plan(batch, tokens, heads, kv_heads, max_len, window);
+    const Kv4Plan pl = kv4_plan(batch, tokens, heads, kv_heads, max_len);
     p.start = start, p.counts = counts, p.start_stride = start_stride ? 1 : 0, p.out = out, p.tokens = tokens, p.heads = heads, p.window = window;
     p.batch = batch, p.cluster = pl.cluster, p.row_tiles = pl.row_tiles, p.row_bytes = head_dim / 2, p.scale_log2 = scale * 1.4426950408889634f;
     p.part_o = static_cast<float*>(workspace);
-    p.part_ml = reinterpret_cast<float2*>(p.part_o + (size_t)pl.stream * 2 * 8 * pl.tiles * head_dim);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + kv4_part_rows(batch, kv_heads, pl) * head_dim);
     const cudaError_t e = pl.tcgen05 ? (head_dim == 128 ? launch_kv4_prefill<128>(p, stream) : launch_kv4_prefill<64>(p, stream))
                           : head_dim == 128 ? (pl.tiles == 1 ? launch_kv4_attend<128, 1>(p, pl.stream, stream) : launch_kv4_attend<128, 2>(p, pl.stream, stream))
                                           : (pl.tiles == 1 ? launch_kv4_attend<64, 1>(p, pl.stream, stream) : launch_kv4_attend<64, 2>(p, pl.stream, stream));

@@ -264,6 +264,47 @@ def test_values_beyond_fp16_among_many_tokens(lib):
     assert torch.equal(out[0].masked_fill(lost[:, None], 0), want[0].masked_fill(lost[:, None], 0))
 
 
+@pytest.mark.parametrize("D,H,K", [(128, 20, 5), (64, 8, 2), (128, 3, 3)])
+@pytest.mark.parametrize("B,T,past,window", [(1, 120, 3000, 0), (2, 257, 1500, 0), (8, 33, 700, 0), (1, 130, 2900, 1), (2, 200, 1000, 64), (1, 300, 2700, 65), (3, 90, 1700, 1000), (1, 1000, 0, 300)])
+def test_attend_keys_in_parts(lib, D, H, K, B, T, past, window):
+    """Many tokens over long caches: the keys of a tile of rows in parts, with parts that no row or some rows see; padded batches; sequences that
+    are shorter than the cache."""
+    cache, k, v = filled(B, K, past + T + 20, D, past + T)
+    q = torch.randn((B, T, H, D), generator=gen(T), device="cuda").to(torch.bfloat16)
+    start = torch.tensor([past, 5, 0, 64, 63, 650, past, 1][:B], device="cuda")
+    check(q, cache, k, v, start, window=window)
+    check(q, cache, k, v, start, counts=torch.tensor([T - 1, 1, 0, T, T // 2, 3, T, 0][:B], device="cuda"), window=window)
+    assert lib.ternaspmm_last_status() == 0
+    start = start.clone()
+    start[0] = cache.max_len - T + 1
+    out = kv4_attend(q, cache, start, window=window)
+    assert out[0].isnan().all() and out[1:].isfinite().all() and lib.ternaspmm_last_status() == 1
+
+
+@pytest.mark.parametrize("window", [0, 30, 500])
+@pytest.mark.parametrize("B,past", [(1, 100), (1, 2300), (2, 2500)])
+def test_bad_scales_among_many_tokens(lib, window, B, past):
+    """Scales that are NaN, infinite or make values beyond 65504: only the rows whose window holds one lose its group; a NaN key loses the row."""
+    T, H, K, D = 300, 8, 2, 128
+    cache, k, v = filled(B, K, past + T + 40, D, 3)
+    q = torch.randn((B, T, H, D), generator=gen(4), device="cuda").to(torch.bfloat16)
+    start = torch.full((B,), past, dtype=torch.int64, device="cuda")
+    want = check(q, cache, k, v, start, window=window)
+    at = past + torch.arange(T, device="cuda")
+    lost = torch.zeros((B, T, H, D), dtype=torch.bool, device="cuda")
+    for b, head, key, group, value in ((0, 1, past + 70, 1, 60000.0), (0, 1, past + 20, 1, float("nan")), (0, 0, past - 20, 3, float("-inf")), (B - 1, 1, past + T - 1, 0, float("nan")),
+                                       (0, 0, past + T, 2, float("nan"))):
+        cache.v_scales[b, head, key, group] = value
+        sees = (at >= key) & ((at < key + window) if window else True)
+        lost[b, sees, 4 * head: 4 * head + 4, 32 * group: 32 * group + 32] = True
+    cache.k_scales[0, 0, past + 150, 1] = float("nan")
+    lost[0, (at >= past + 150) & ((at < past + 150 + window) if window else True), :4] = True
+    out = kv4_attend(q, cache, start, window=window)
+    assert torch.equal(out.isnan(), lost)
+    assert torch.equal(out.masked_fill(lost, 0), want.masked_fill(lost, 0))
+    assert lib.ternaspmm_last_status() == 0
+
+
 def test_infinite_and_nan_inputs_stay_in_their_group(lib):
     cache = KV4Cache.empty(1, 1, 64, 128)
     x = torch.ones((1, 1, 1, 128), device="cuda", dtype=torch.bfloat16)
@@ -308,6 +349,29 @@ def test_two_graphs_and_streams(lib):
             outs.append(kv4_attend(x, cache, s))
     for s in start:
         s.copy_(torch.randint(0, L, (B,), device="cuda"))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for o, x, s in zip(outs, q, start):
+        assert torch.equal(o, check(x, cache, k, v, s))
+
+
+def test_two_graphs_of_many_tokens(lib):
+    """The same with the keys in parts, whose results meet in a workspace."""
+    B, T, H, K, D, L = 2, 80, 8, 2, 128, 2048
+    cache, k, v = filled(B, K, L, D, 7)
+    q = [torch.randn((B, T, H, D), generator=gen(i), device="cuda").to(torch.bfloat16) for i in range(2)]
+    start = [torch.tensor([900, 1700], device="cuda"), torch.tensor([L - T, 17], device="cuda")]
+    kv4_attend(q[0], cache, start[0])
+    graphs, outs, streams = [torch.cuda.CUDAGraph() for _ in q], [], [torch.cuda.Stream() for _ in q]
+    for g, x, s in zip(graphs, q, start):
+        with torch.cuda.graph(g):
+            outs.append(kv4_attend(x, cache, s))
+    for s in start:
+        s.copy_(torch.randint(0, L - T, (B,), device="cuda"))
     torch.cuda.synchronize()
     for _ in range(20):
         for g, st in zip(graphs, streams):
