@@ -51,10 +51,12 @@ __device__ __forceinline__ uint32_t lp_order(float x) {
 __device__ __forceinline__ float lp_value(uint32_t o) {
     return o == 0xffffffffu ? __int_as_float(0x7fffffff) : __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
-// larger value first, then the lower index
-__device__ __forceinline__ unsigned long long lp_key(float x, int i) { return (unsigned long long)lp_order(x) << 32 | (0xffffffffu - (uint32_t)i); }
+// larger value first, then the lower index; neither 0 nor the largest number
+__device__ __forceinline__ unsigned long long lp_key(float x, int i) { return (unsigned long long)lp_order(x) << 32 | (0xfffffffeu - (uint32_t)i); }
+__device__ __forceinline__ long long lp_token(unsigned long long key) { return 0xfffffffeu - (uint32_t)key; }
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr double kOverLog2e = 1.0 / kLog2e;                       // (of the rounded one: divisions in 64 bits took as long as a short row's sums)
 
 // 16 bytes of logits
 template <typename T> struct LpVec;
@@ -146,6 +148,113 @@ struct LpPart {
     }
 };
 
+// A warp's sums over a run of elements: l, w of every lane's, relative to 2^ref; `near`: ref is a float that takes the short way, up to elements of `limit`.
+template <typename T>
+struct LpRun {
+    double ref = -INFINITY;
+    float2 l = make_float2(0.f, 0.f), w = l;
+    bool near = false;
+    float limit = 0.f;
+
+    // Adds the first n vectors of x16 and, where edge >= 0, xe; tm is the largest of them (NaN aside).  pl: the lane's own l, NaN where one of its
+    // elements is NaN or +inf; again(j) reads vector j once more.
+    template <typename F>
+    __device__ __forceinline__ void add(const LpVec<T> (&x16)[kLpVecs], int n, float tm, int edge, float xe, float2& pl, float2& pw, F again) {
+        constexpr int V = LpVec<T>::N;
+        auto add_all = [&](float r, float2& sl, float2& sw) {      // t = x log2(e) - r
+            const float2 e2 = make_float2(kLog2e, kLog2e), nr = make_float2(-r, -r);
+#pragma unroll
+            for (int j = 0; j < kLpVecs; ++j) {
+                if (j >= n) break;
+                float x[V];
+                x16[j].floored().get(x);
+#pragma unroll
+                for (int i = 0; i < V; i += 2) {
+                    const float2 t = f32x2_fma(make_float2(x[i], x[i + 1]), e2, nr), e = make_float2(ex2_approx(t.x), ex2_approx(t.y));
+                    sl = f32x2_add(sl, e), sw = f32x2_fma(e, t, sw);
+                }
+            }
+            if (edge >= 0) {
+                const float t = fmaf(xe < -1e37f ? -1e37f : xe, kLog2e, -r), e = ex2_approx(t);
+                sl.x += e, sw.x = fmaf(e, t, sw.x);
+            }
+        };
+        if (near && !__any_sync(0xffffffffu, tm > limit)) {
+            add_all((float)ref, pl, pw);
+            l = f32x2_add(l, pl), w = f32x2_add(w, pw);
+        } else {                                                   // the first part of a run, or one with much larger elements
+            float m = tm;
+#pragma unroll
+            for (int j = 16; j; j >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, j));
+            double part_ref = (double)m * kLog2e;
+            if (lp_near<T>(m)) {
+                part_ref = m * kLog2e;                             // (as rounded to fp32)
+                add_all((float)part_ref, pl, pw);
+            } else {                                               // a maximum of the type's largest or lowest order, or infinite: differences first
+                auto far = [&](float x) {
+                    const float t = fmaxf((x - m) * kLog2e, -200.f), e = x == -INFINITY ? 0.f : ex2_approx((x - m) * kLog2e);
+                    pl.x += e, pw.x = fmaf(e, t, pw.x);
+                };
+#pragma unroll 1
+                for (int j = 0; j < n; ++j) {
+                    float x[V];
+                    again(j).get(x);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) far(x[i]);
+                }
+                if (edge >= 0) far(xe);
+            }
+            // (part_ref of -inf: nothing but -inf and NaN)
+            const double to = fmax(ref, part_ref);
+            const float ds = ref == -INFINITY ? 0.f : (float)(ref - to), dp = part_ref == -INFINITY ? 0.f : (float)(part_ref - to);
+            const float fs = ex2_approx(ds), fp = ex2_approx(dp), cs = fmaxf(ds, -200.f), cp = fmaxf(dp, -200.f);
+            w.x = (w.x + w.y + (l.x + l.y) * cs) * fs + (pw.x + pw.y + (pl.x + pl.y) * cp) * fp, w.y = 0.f;
+            l.x = (l.x + l.y) * fs + (pl.x + pl.y) * fp, l.y = 0.f;
+            ref = to;
+            near = fabs(ref) < 1.4e36 && lp_near<T>((float)(ref * 0.69314718)) && (double)(float)ref == ref;
+            limit = (float)((ref + 60) * 0.69314718);              // (2^60 times as many elements as a row has fit into fp32)
+        }
+    }
+};
+
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+    for (int j = 16; j; j >>= 1) x += __shfl_xor_sync(0xffffffffu, x, j);
+    return x;
+}
+
+// Log probability of x beside a sum of 2^(ref + ll) (differences first: ll is nothing beside the reference of a row of the type's lowest value);
+// rounding does not take it above 0.
+__device__ __forceinline__ float lp_of(float x, double ref, float ll) {
+    const float lp = (float)((((double)x * (double)kLog2e - ref) - ll) * kOverLog2e);
+    return lp > 0.f ? 0.f : lp;
+}
+// A row's results but for the alternatives.
+__device__ __forceinline__ void lp_finish(const LogprobParams& p, long long r, long long target, float xt, double ref, float ll, float l, float w) {
+    float lp = lp_of(xt, ref, ll);
+    if (target < 0) lp = 0.f;                                      // no token
+    if (target >= p.vocab) {
+        lp = __int_as_float(0x7fffffff);
+        *p.status = 1;
+    }
+    p.logprob[r] = lp;
+    const float h = (ll - w / l) * kLn2;
+    p.entropy[r] = h < 0.f ? 0.f : h;
+    // in two parts, for the gradient
+    const float hi = (float)(ref * kOverLog2e);
+    p.lse[2 * r] = hi, p.lse[2 * r + 1] = (float)(((ref - (double)hi * (double)kLog2e) + ll) * kOverLog2e);
+}
+// Of `mine` of all lanes, the k-th largest (k <= 32).
+__device__ __forceinline__ uint32_t lp_kth(uint32_t mine, int k, int lane) {
+    int rank = 0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+        const uint32_t other = __shfl_sync(0xffffffffu, mine, j);
+        rank += other > mine || (other == mine && j < lane);
+    }
+    return __shfl_sync(0xffffffffu, mine, __ffs(__ballot_sync(0xffffffffu, rank == k - 1)) - 1);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) logprob_kernel(const LogprobParams p) {
     using Vec16 = LpVec<T>;
@@ -191,11 +300,7 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) logprob_kernel(const
     const unsigned r_now = run / p.lists, next = run + gridDim.x;
     const int first = (int)(run - r_now * p.lists) * p.run, count = min(p.run, p.parts - first);
     bool full = false;
-    // the warp's sums: l, w of every lane's elements, relative to 2^ref; `near`: ref is a float that takes the short way, up to elements of `limit`
-    double ref = -INFINITY;
-    float2 l = make_float2(0.f, 0.f), w = l;
-    bool near = false;
-    float limit = 0.f;
+    LpRun<T> sums;
     LpPart<T> at(p, r_now, first);
 #pragma unroll 1
     for (int k = 0; k < count; ++k, buf ^= 1, ++at.part, at.first += kLpThreads * kLpVecs) {
@@ -225,58 +330,7 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) logprob_kernel(const
             if (vm > above) hits |= 1u << j;
         }
         float2 pl = make_float2(0.f, 0.f), pw = pl;
-        auto add_all = [&](float r, float2& sl, float2& sw) {      // t = x log2(e) - r
-            const float2 e2 = make_float2(kLog2e, kLog2e), nr = make_float2(-r, -r);
-#pragma unroll
-            for (int j = 0; j < kLpVecs; ++j) {
-                float x[V];
-                x16[j].floored().get(x);
-#pragma unroll
-                for (int i = 0; i < V; i += 2) {
-                    const float2 t = f32x2_fma(make_float2(x[i], x[i + 1]), e2, nr), e = make_float2(ex2_approx(t.x), ex2_approx(t.y));
-                    sl = f32x2_add(sl, e), sw = f32x2_fma(e, t, sw);
-                }
-            }
-            if (edge >= 0) {
-                const float t = fmaf(xe < -1e37f ? -1e37f : xe, kLog2e, -r), e = ex2_approx(t);
-                sl.x += e, sw.x = fmaf(e, t, sw.x);
-            }
-        };
-        if (near && !__any_sync(0xffffffffu, tm > limit)) {
-            add_all((float)ref, pl, pw);
-            l = f32x2_add(l, pl), w = f32x2_add(w, pw);
-        } else {                                                   // the first part of a run, or one with much larger elements
-            float m = tm;
-#pragma unroll
-            for (int j = 16; j; j >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, j));
-            double part_ref = (double)m * kLog2e;
-            if (lp_near<T>(m)) {
-                part_ref = m * kLog2e;                             // (as rounded to fp32)
-                add_all((float)part_ref, pl, pw);
-            } else {                                               // a maximum of the type's largest or lowest order, or infinite: differences first
-                auto add = [&](float x) {
-                    const float t = fmaxf((x - m) * kLog2e, -200.f), e = x == -INFINITY ? 0.f : ex2_approx((x - m) * kLog2e);
-                    pl.x += e, pw.x = fmaf(e, t, pw.x);
-                };
-#pragma unroll 1
-                for (int j = 0; j < kLpVecs; ++j) {
-                    float x[V];
-                    Vec16{lds128(src + j * 512)}.get(x);
-#pragma unroll
-                    for (int i = 0; i < V; ++i) add(x[i]);
-                }
-                if (edge >= 0) add(xe);
-            }
-            // (part_ref of -inf: nothing but -inf and NaN)
-            const double to = fmax(ref, part_ref);
-            const float ds = ref == -INFINITY ? 0.f : (float)(ref - to), dp = part_ref == -INFINITY ? 0.f : (float)(part_ref - to);
-            const float fs = ex2_approx(ds), fp = ex2_approx(dp), cs = fmaxf(ds, -200.f), cp = fmaxf(dp, -200.f);
-            w.x = (w.x + w.y + (l.x + l.y) * cs) * fs + (pw.x + pw.y + (pl.x + pl.y) * cp) * fp, w.y = 0.f;
-            l.x = (l.x + l.y) * fs + (pl.x + pl.y) * fp, l.y = 0.f;
-            ref = to;
-            near = fabs(ref) < 1.4e36 && lp_near<T>((float)(ref * 0.69314718)) && (double)(float)ref == ref;
-            limit = (float)((ref + 60) * 0.69314718);              // (2^60 times as many elements as a row has fit into fp32)
-        }
+        sums.add(x16, kLpVecs, tm, edge, xe, pl, pw, [&](int j) { return Vec16{lds128(src + j * 512)}; });
         if (p.top == 0) continue;
 
         // ---- candidates for the most probable tokens
@@ -299,14 +353,7 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) logprob_kernel(const
             for (int j = 1; j < 8; j <<= 1) gm = max(gm, __shfl_xor_sync(0xffffffffu, gm, j));
             if ((lane & 7) == 0) groups[warp * 4 + (lane >> 3)] = gm;
             __syncthreads();
-            const uint32_t v = groups[lane];
-            int rank = 0;
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-                const uint32_t other = __shfl_sync(0xffffffffu, v, j);
-                rank += other > v || (other == v && j < lane);
-            }
-            bound = __shfl_sync(0xffffffffu, v, __ffs(__ballot_sync(0xffffffffu, rank == p.top - 1)) - 1);   // that p.top of the groups reach
+            bound = lp_kth(groups[lane], p.top, lane);             // that p.top of the groups reach
             if (u >= bound) {
                 const float bf = lp_value(bound);
 #pragma unroll
@@ -367,10 +414,8 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) logprob_kernel(const
         }
     }
     {
-        float sl = l.x + l.y, sw = w.x + w.y;
-#pragma unroll
-        for (int j = 16; j; j >>= 1) sl += __shfl_xor_sync(0xffffffffu, sl, j), sw += __shfl_xor_sync(0xffffffffu, sw, j);
-        if (lane == 0) p.sums[(size_t)run * kLpWarps + warp] = {ref, ok ? sl : __int_as_float(0x7fffffff), sw};
+        const float sl = warp_sum(sums.l.x + sums.l.y), sw = warp_sum(sums.w.x + sums.w.y);
+        if (lane == 0) p.sums[(size_t)run * kLpWarps + warp] = {sums.ref, ok ? sl : __int_as_float(0x7fffffff), sw};
     }
     if (p.top == 0) continue;
     unsigned long long* keys = p.keys + (size_t)run * p.top;
@@ -418,11 +463,163 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) logprob_kernel(const
     if (!ok && lane == 0) atomicExch(p.status, ST_WAIT_TIMEOUT);
 }
 
-// Log probability of x beside a sum of 2^(ref + ll) (differences first: ll is nothing beside the reference of a row of the type's lowest value);
-// rounding does not take it above 0.
-__device__ __forceinline__ float lp_of(float x, double ref, float ll) {
-    const float lp = (float)((((double)x * (double)kLog2e - ref) - ll) / (double)kLog2e);
-    return lp > 0.f ? 0.f : lp;
+// Rows of at most one part, a warp each and nothing between the warps: 100,000 rows of 300 logits took 754 us with a CTA for each, which
+// left most of it idle.  A warp has up to 4 KB of its row in registers at a time.  The k-th largest of the lanes' maxima is the
+// bound for the alternatives of the first 4 KB, the k-th largest element so far that for the next ones.
+constexpr int kLpRowCandidates = 256, kLpRanked = 64;
+template <typename T>
+__global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) logprob_rows_kernel(const LogprobParams p) {
+    using Vec16 = LpVec<T>;
+    constexpr int V = Vec16::N;
+    __shared__ unsigned long long lists[kLpWarps][kLpRowCandidates];
+    __shared__ int counts[kLpWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const unsigned r = blockIdx.x * kLpWarps + warp;
+    if (r >= (unsigned)p.rows) return;                             // (no barrier of the CTA below)
+    unsigned long long* cand = lists[warp];
+    LpPart<T> at(p, r, 0);
+    const long long target = p.targets[r];
+    const float xt = target >= 0 && target < p.vocab ? Elem<T>::get(at.row[target]) : 0.f;
+    if (lane == 0) counts[warp] = 0;
+    LpRun<T> sums;
+    uint32_t bound = 0;
+    bool full = false;
+#pragma unroll 1
+    for (int k = 0; k == 0 || at.first < at.vecs; ++k, at.first += 32 * kLpVecs) {
+        const int edge = k == 0 ? at.edge(lane) : -1, n = min(kLpVecs, (at.vecs - at.first + 31) / 32);
+        auto again = [&](int j) { return at.has(j, lane) ? Vec16{ldg_128(at.row + at.index(j, lane))} : Vec16{make_uint4(Vec16::none, Vec16::none, Vec16::none, Vec16::none)}; };
+        Vec16 x16[kLpVecs];
+#pragma unroll
+        for (int j = 0; j < kLpVecs; ++j)
+            if (j < n) x16[j] = again(j);
+        const float xe = edge >= 0 ? Elem<T>::get(at.row[edge]) : -INFINITY;
+        float tm = xe;                                             // this lane's maximum (NaN aside)
+        uint32_t hits = 0;                                         // vectors with an element above the bound so far
+        const float above = k > 0 ? lp_value(bound) : INFINITY;
+#pragma unroll
+        for (int j = 0; j < kLpVecs; ++j) {
+            if (j >= n) break;
+            const float vm = x16[j].max();
+            tm = fmaxf(tm, vm);
+            if (vm > above) hits |= 1u << j;
+        }
+        float2 pl = make_float2(0.f, 0.f), pw = pl;
+        sums.add(x16, n, tm, edge, xe, pl, pw, again);
+        if (p.top == 0 || full) continue;
+
+        const float own = pl.x + pl.y;
+        const bool odd = own != own;                               // NaN or +inf among this lane's elements: which, the sum does not tell
+        if (k == 0) {
+            uint32_t u = lp_order(tm);
+            if (odd) {
+                u = lp_order(xe);
+#pragma unroll 1
+                for (int j = 0; j < n; ++j) {
+                    float x[V];
+                    again(j).get(x);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) u = max(u, lp_order(x[i]));
+                }
+            }
+            bound = lp_kth(u, p.top, lane);
+            if (u >= bound) {
+                const float bf = lp_value(bound);
+#pragma unroll
+                for (int j = 0; j < kLpVecs; ++j)
+                    if (j < n && !(x16[j].max() < bf)) hits |= 1u << j;
+            }
+        }
+        if (odd && bound != 0xffffffffu) hits = (1u << n) - 1;
+        const uint32_t least = bound + (k > 0 ? 1u : 0u);          // (as in logprob_kernel)
+        const float bf = lp_value(least);
+        auto push = [&](float x, int i) {
+            if (lp_order(x) >= least) {
+                const int to = atomicAdd(&counts[warp], 1);
+                if (to < kLpRowCandidates) cand[to] = lp_key(x, i);
+            }
+        };
+        __syncwarp();
+        if (bound == 0xffffffffu && k > 0) hits = 0;               // (nothing is above p.top times NaN)
+        while (hits) {
+            const int j = __ffs(hits) - 1;
+            hits &= hits - 1;
+            if (!at.has(j, lane)) continue;
+            float x[V];
+            again(j).get(x);
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (!(x[i] < bf)) push(x[i], at.index(j, lane) + i);
+        }
+        if (edge >= 0) push(xe, edge);
+        __syncwarp();
+        int c = counts[warp];
+        if (c > kLpRowCandidates) {                                // many elements at the bound or above it: found at the end
+            full = true;
+            continue;
+        }
+        if (c > kLpRanked) {                                       // a border that leaves p.top .. kLpRanked of them, by halving: keys differ
+            unsigned long long key[kLpRowCandidates / 32], lo = 0ull, hi = ~0ull;
+#pragma unroll
+            for (int i = 0; i < kLpRowCandidates / 32; ++i) key[i] = i * 32 + lane < c ? cand[i * 32 + lane] : 0ull;
+            if (least) lo = ((unsigned long long)least << 32) - 1; // (all are above it)
+            int over = c;
+#pragma unroll 1
+            for (int step = 0; step < 64 && (over > kLpRanked || over < p.top); ++step) {
+                const unsigned long long mid = lo + (hi - lo) / 2;
+                int mine = 0;
+#pragma unroll
+                for (int i = 0; i < kLpRowCandidates / 32; ++i) mine += key[i] > mid;
+                over = __reduce_add_sync(0xffffffffu, mine);
+                if (over > kLpRanked) lo = mid;
+                else hi = mid;                                     // (the border itself, if this ends it)
+            }
+            __syncwarp();
+            c = 0;
+#pragma unroll
+            for (int i = 0; i < kLpRowCandidates / 32; ++i) {
+                const uint32_t kept = __ballot_sync(0xffffffffu, key[i] > hi);
+                if (key[i] > hi) cand[c + __popc(kept & ((1u << lane) - 1))] = key[i];
+                c += __popc(kept);
+            }
+            __syncwarp();
+        }
+        const unsigned long long k0 = lane < c ? cand[lane] : 0ull, k1 = lane + 32 < c ? cand[lane + 32] : 0ull;
+        int rank0 = 0, rank1 = 0;
+        for (int i = 0; i < c; ++i) rank0 += cand[i] > k0, rank1 += cand[i] > k1;
+        __syncwarp();
+        if (k0 && rank0 < p.top) cand[rank0] = k0;
+        if (k1 && rank1 < p.top) cand[rank1] = k1;
+        if (lane == 0) counts[warp] = min(c, p.top);
+        __syncwarp();
+        if (c >= p.top) bound = (uint32_t)(cand[p.top - 1] >> 32);
+    }
+    double ref = sums.ref;                                         // (the same in all lanes)
+    const float l = warp_sum(sums.l.x + sums.l.y), w = warp_sum(sums.w.x + sums.w.y);
+    const float ll = ref == -INFINITY ? __int_as_float(0x7fffffff) : log2f(l);
+    if (lane == 0) lp_finish(p, r, target, xt, ref, ll, l, w);
+    if (p.top == 0) return;
+    unsigned long long key = lane < p.top ? cand[lane] : 0ull;
+    if (full) {                                                    // a pass over the row for each place
+        unsigned long long last = ~0ull;
+        for (int place = 0; place < p.top; ++place) {
+            unsigned long long top = 0;
+            for (int i = lane; i < p.vocab; i += 32) {
+                const unsigned long long y = lp_key(Elem<T>::get(at.row[i]), i);
+                if (y < last && y > top) top = y;
+            }
+#pragma unroll
+            for (int j = 16; j; j >>= 1) {
+                const unsigned long long other = __shfl_xor_sync(0xffffffffu, top, j);
+                top = other > top ? other : top;
+            }
+            last = top;
+            if (lane == place) key = top;
+        }
+    }
+    if (lane < p.top) {
+        p.top_logprob[(size_t)r * p.top + lane] = lp_of(lp_value((uint32_t)(key >> 32)), ref, ll);
+        p.top_token[(size_t)r * p.top + lane] = lp_token(key);
+    }
 }
 
 // Joins a row's parts: a warp per row.
@@ -454,20 +651,7 @@ __global__ void __launch_bounds__(32) logprob_join_kernel(const LogprobParams p)
     for (int j = 16; j; j >>= 1) l += __shfl_xor_sync(0xffffffffu, l, j), w += __shfl_xor_sync(0xffffffffu, w, j);
     // log2 of the sum of 2^(x log2(e)); the units are those of log2(e) as rounded to fp32.  Without a finite logit it is NaN
     const float ll = ref == -INFINITY ? __int_as_float(0x7fffffff) : log2f(l);
-    if (lane == 0) {
-        float lp = lp_of(xt, ref, ll);
-        if (target < 0) lp = 0.f;                                  // no token
-        if (target >= p.vocab) {
-            lp = __int_as_float(0x7fffffff);
-            *p.status = 1;
-        }
-        p.logprob[r] = lp;
-        const float h = (ll - w / l) * kLn2;
-        p.entropy[r] = h < 0.f ? 0.f : h;
-        // in two parts, for the gradient
-        const float hi = (float)(ref / (double)kLog2e);
-        p.lse[2 * r] = hi, p.lse[2 * r + 1] = (float)(((ref - (double)hi * (double)kLog2e) + ll) / (double)kLog2e);
-    }
+    if (lane == 0) lp_finish(p, r, target, xt, ref, ll, l, w);
     __syncwarp();
     for (int k = 0; k < p.top; ++k) {                              // the lists' heads against each other
         unsigned long long key = 0;
@@ -485,7 +669,7 @@ __global__ void __launch_bounds__(32) logprob_join_kernel(const LogprobParams p)
         if (key == top) {                                          // (keys differ: one lane; top <= vocab: none is 0)
             ++place[from];
             p.top_logprob[r * p.top + k] = lp_of(lp_value((uint32_t)(key >> 32)), ref, ll);
-            p.top_token[r * p.top + k] = 0xffffffffu - (uint32_t)key;
+            p.top_token[r * p.top + k] = lp_token(key);
         }
         __syncwarp();
     }
@@ -497,14 +681,15 @@ struct LogprobGradParams {
     const long long* targets;
     const float *lse, *entropy, *g_logprob, *g_entropy;            // either gradient may be null
     void* grad;                                                    // contiguous [rows][vocab]
-    int vocab;
+    int rows, vocab;
 };
 
-// d/dx_j = g (delta_jt - p_j) - h p_j (log p_j + H).  One CTA per row and part of it.
+// d/dx_j = g (delta_jt - p_j) - h p_j (log p_j + H).  A CTA per row and part of it, or 256 / threads rows of one part.
 template <typename T>
-__global__ void __launch_bounds__(256) logprob_grad_kernel(const LogprobGradParams p, int parts) {
+__global__ void __launch_bounds__(256) logprob_grad_kernel(const LogprobGradParams p, int parts, int threads) {
     constexpr int V = 16 / sizeof(T);
-    const size_t r = blockIdx.x / parts;
+    const size_t r = blockIdx.x / parts * (256u / threads) + threadIdx.x / threads;
+    if (r >= (size_t)p.rows) return;
     const int part = blockIdx.x % parts;
     const T* row = static_cast<const T*>(p.logits) + (long long)r * p.ld;
     T* out = static_cast<T*>(p.grad) + r * (size_t)p.vocab;
@@ -519,7 +704,7 @@ __global__ void __launch_bounds__(256) logprob_grad_kernel(const LogprobGradPara
     const bool same = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
     const int head = same ? min(p.vocab, (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(T)) : 0;
     const int vecs = same ? (p.vocab - head) / V : 0;
-    const int tid = part * 256 + threadIdx.x, all = parts * 256;
+    const int tid = part * 256 + threadIdx.x % threads, all = parts * threads;
     for (int i = tid; i < vecs; i += all) {
         const int j0 = head + i * V;
         const Vec<T, V> x = *reinterpret_cast<const Vec<T, V>*>(row + j0);

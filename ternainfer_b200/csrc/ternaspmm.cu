@@ -1463,11 +1463,19 @@ static bool logprob_shape(int rows, int vocab, int type, int top) {
 
 extern "C" long long ternaspmm_token_logprobs_workspace(int rows, int vocab, int type, int top) {
     if (!logprob_shape(rows, vocab, type, top)) return -1;
+    if (logprob_parts(vocab, type) == 1) return 16;                // (logprob_rows_kernel has none)
     return (long long)rows * logprob_parts(vocab, type) * (kLpWarps * (int)sizeof(LpSums) + 8 * top);
 }
 
 template <typename T>
 static cudaError_t launch_logprobs(const LogprobParams& p, cudaStream_t stream) {
+    if (p.parts == 1) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)((p.rows + kLpWarps - 1) / kLpWarps), 1, 1);
+        cfg.blockDim = dim3(kLpThreads, 1, 1);
+        cfg.stream = stream;
+        return cudaLaunchKernelEx(&cfg, logprob_rows_kernel<T>, p);
+    }
     static bool done[64] = {false};
     int dev = 0;
     cudaGetDevice(&dev);
@@ -1526,14 +1534,15 @@ extern "C" int ternaspmm_token_logprobs_grad(const void* logits, long long ld, i
     if (rows < 1 || vocab < 1 || ld < vocab || type < 0 || type > 2) return t_host_status = ST_BAD_SHAPE;
     if (!logits || !targets || !lse || !entropy || !grad || (reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(grad)) % (type == 2 ? 4 : 2))
         return t_host_status = ST_BAD_POINTER;
-    LogprobGradParams p = {logits, ld, targets, lse, entropy, g_logprob, g_entropy, grad, vocab};
-    const int parts = (vocab + 8191) / 8192;
-    if ((long long)rows * parts > 0x7fffffffll) return t_host_status = ST_BAD_SHAPE;
+    LogprobGradParams p = {logits, ld, targets, lse, entropy, g_logprob, g_entropy, grad, rows, vocab};
+    const int parts = (vocab + 8191) / 8192, threads = vocab <= 2048 ? 32 : 256;
+    const long long ctas = parts == 1 ? ((long long)rows + 256 / threads - 1) / (256 / threads) : (long long)rows * parts;
+    if (ctas > 0x7fffffffll) return t_host_status = ST_BAD_SHAPE;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((long long)rows * parts), 1, 1);
+    cfg.gridDim = dim3((unsigned)ctas, 1, 1);
     cfg.blockDim = dim3(256, 1, 1);
     cfg.stream = stream;
-    if (cudaLaunchKernelEx(&cfg, type == 0 ? logprob_grad_kernel<__nv_bfloat16> : type == 1 ? logprob_grad_kernel<__half> : logprob_grad_kernel<float>, p, parts) != cudaSuccess)
+    if (cudaLaunchKernelEx(&cfg, type == 0 ? logprob_grad_kernel<__nv_bfloat16> : type == 1 ? logprob_grad_kernel<__half> : logprob_grad_kernel<float>, p, parts, threads) != cudaSuccess)
         t_host_status = ST_LAUNCH;
     checkLastCudaError(__LINE__);
     return t_host_status;

@@ -91,6 +91,54 @@ def test_rows_without_a_distribution(lib):
     assert lib.ternaspmm_last_status() == 0
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [40, 300, 1031, 5000, 30000, 150000])
+def test_rows_of_one_kind(lib, dtype, V):
+    """More candidates than are kept: rows of NaN, of one value, of the lowest value, of -inf but for a few; a NaN and an infinity among others."""
+    g = gen(V)
+    x = torch.randn((9, V), generator=g, device="cuda").to(dtype)
+    x[0], x[1], x[2], x[3] = float("nan"), 0.5, torch.finfo(dtype).min, float("-inf")
+    x[3, 11], x[3, V - 1] = 1.0, 2.0
+    x[4, V // 2] = float("nan")
+    x[5, 0] = float("nan")
+    x[6, [0, V - 1]] = float("inf")
+    x[7, 3:] = x[7, 3]
+    t = torch.zeros(9, dtype=torch.int64, device="cuda")
+    for top in (1, 7, 32):
+        got = token_logprobs(x, t, top)
+        y = x.float()
+        sort_key = torch.where(y.isnan(), torch.full_like(y, float("inf")), torch.where(y == float("inf"), torch.full_like(y, torch.finfo(torch.float32).max), y))
+        order = torch.sort(sort_key, dim=-1, descending=True, stable=True)[1]
+        assert torch.equal(got.top_token, order[:, :top])
+    for r in (1, 2, 3, 7, 8):
+        check(x[r: r + 1], t[r: r + 1] + (11 if r == 3 else 0), 5)
+    assert got.logprob[[0, 4, 5, 6]].isnan().all() and got.entropy[[0, 4, 5, 6]].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_short_rows(lib, dtype):
+    """More rows than are at work at once, of lengths around those where a warp goes on to its next vectors; rows at any alignment."""
+    g = gen(2)
+    for N, V, step in ((5000, 131, 131), (4001, 255, 260), (700, 2050, 2051), (300, 8200, 8200), (64, 16391, 16400)):
+        x = (3 * torch.randn((N, step), generator=g, device="cuda")).to(dtype)[:, :V]
+        t = torch.randint(-1, V, (N,), generator=g, device="cuda")
+        for top in (0, 20, 32):
+            check(x, t, top)
+        y = x.detach().clone().requires_grad_()
+        got = token_logprobs(y, t)
+        w = torch.randn(N, generator=g, device="cuda")
+        grad, = torch.autograd.grad(got.logprob, y, w)
+        p = torch.softmax(x.double(), -1)
+        live = (t >= 0).double()[:, None]
+        hot = torch.nn.functional.one_hot(t.clamp(0), V).double()
+        want = (hot - p) * live * w[:, None].double()
+        # p is off by 2^-18 of itself (its exponent holds up to 2^5, rounded three times, and the log of the sum); then one rounding
+        eps = torch.finfo(dtype).eps / 2
+        tiny = {torch.float16: 2.0 ** -25}.get(dtype, 0.0)
+        assert ((grad.double() - want).abs() <= w.abs()[:, None].double() * live * p * 2.0 ** -18 * (1 + eps) + want.abs() * (eps + 2.0 ** -22) + tiny).all()
+    assert lib.ternaspmm_last_status() == 0
+
+
 def test_targets(lib):
     """No token, tokens outside of the vocabulary, any shape, rows apart from each other, targets of any strides."""
     g = gen(2)
