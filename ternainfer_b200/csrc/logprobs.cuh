@@ -255,6 +255,20 @@ __device__ __forceinline__ uint32_t lp_kth(uint32_t mine, int k, int lane) {
     return __shfl_sync(0xffffffffu, mine, __ffs(__ballot_sync(0xffffffffu, rank == k - 1)) - 1);
 }
 
+// The same of two of every lane.
+__device__ __forceinline__ uint32_t lp_kth_of_64(uint32_t a, uint32_t b, int k, int lane) {
+    int rank_a = a < b, rank_b = a >= b;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+        const uint32_t x = __shfl_sync(0xffffffffu, a, j), y = __shfl_sync(0xffffffffu, b, j);
+        if (j == lane) continue;
+        rank_a += (x > a || (x == a && j < lane)) + (y > a || (y == a && j < lane));
+        rank_b += (x > b || (x == b && j < lane)) + (y > b || (y == b && j < lane));
+    }
+    const uint32_t in_a = __ballot_sync(0xffffffffu, rank_a == k - 1), in_b = __ballot_sync(0xffffffffu, rank_b == k - 1);   // (one lane, one of its two)
+    return __shfl_sync(0xffffffffu, in_a ? a : b, __ffs(in_a ? in_a : in_b) - 1);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) logprob_kernel(const LogprobParams p) {
     using Vec16 = LpVec<T>;
@@ -463,9 +477,12 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) logprob_kernel(const
     if (!ok && lane == 0) atomicExch(p.status, ST_WAIT_TIMEOUT);
 }
 
-// Rows of at most one part, a warp each and nothing between the warps: 100,000 rows of 300 logits took 754 us with a CTA for each, which
-// left most of it idle.  A warp has up to 4 KB of its row in registers at a time.  The k-th largest of the lanes' maxima is the
-// bound for the alternatives of the first 4 KB, the k-th largest element so far that for the next ones.
+// Short rows, a warp each and nothing between the warps: 100,000 rows of 300 fp32 logits take 89 us (1.3 TB/s; 754 with a CTA for each, which left
+// most of it idle), 8,000 of 5,000 bf16 28 us (2.8 TB/s).  What bounds the shortest is the chain of loads, sums and logarithm of a row, 24 of
+// them at work on an SM.  A warp has up to 4 KB of its row in registers at a time.  The k-th largest of the lanes' maxima is the bound for the
+// alternatives of the first 4 KB, the k-th largest element so far that for the next ones.  Above the least of 32 maxima (k = 32) one row in a
+// hundred has more than 256 elements, and takes ten times as long; so for many alternatives a lane has two groups, its even and its odd vectors:
+// 44 elements on average are above the 32nd of 64 (300 rows of 4,000: 104 -> 19 us; with k = 5 the 64 cost 12.2 us and the 32 10.4).
 constexpr int kLpRowCandidates = 256, kLpRanked = 64;
 template <typename T>
 __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) logprob_rows_kernel(const LogprobParams p) {
@@ -493,16 +510,17 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) logprob_rows_kernel(
         for (int j = 0; j < kLpVecs; ++j)
             if (j < n) x16[j] = again(j);
         const float xe = edge >= 0 ? Elem<T>::get(at.row[edge]) : -INFINITY;
-        float tm = xe;                                             // this lane's maximum (NaN aside)
+        float tm2[2] = {xe, -INFINITY};                            // the maxima of this lane's groups (NaN aside)
         uint32_t hits = 0;                                         // vectors with an element above the bound so far
         const float above = k > 0 ? lp_value(bound) : INFINITY;
 #pragma unroll
         for (int j = 0; j < kLpVecs; ++j) {
             if (j >= n) break;
             const float vm = x16[j].max();
-            tm = fmaxf(tm, vm);
+            tm2[j & 1] = fmaxf(tm2[j & 1], vm);
             if (vm > above) hits |= 1u << j;
         }
+        const float tm = fmaxf(tm2[0], tm2[1]);
         float2 pl = make_float2(0.f, 0.f), pw = pl;
         sums.add(x16, n, tm, edge, xe, pl, pw, again);
         if (p.top == 0 || full) continue;
@@ -510,9 +528,9 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) logprob_rows_kernel(
         const float own = pl.x + pl.y;
         const bool odd = own != own;                               // NaN or +inf among this lane's elements: which, the sum does not tell
         if (k == 0) {
-            uint32_t u = lp_order(tm);
-            if (odd) {
-                u = lp_order(xe);
+            uint32_t u = lp_order(tm2[0]), u1 = lp_order(tm2[1]);
+            if (odd) {                                             // (its largest speaks for the lane)
+                u = lp_order(xe), u1 = lp_order(-INFINITY);
 #pragma unroll 1
                 for (int j = 0; j < n; ++j) {
                     float x[V];
@@ -521,8 +539,8 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) logprob_rows_kernel(
                     for (int i = 0; i < V; ++i) u = max(u, lp_order(x[i]));
                 }
             }
-            bound = lp_kth(u, p.top, lane);
-            if (u >= bound) {
+            bound = p.top > 24 ? lp_kth_of_64(u, u1, p.top, lane) : lp_kth(max(u, u1), p.top, lane);
+            if (max(u, u1) >= bound) {
                 const float bf = lp_value(bound);
 #pragma unroll
                 for (int j = 0; j < kLpVecs; ++j)

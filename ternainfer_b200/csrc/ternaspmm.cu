@@ -1457,19 +1457,26 @@ static int logprob_parts(int vocab, int type) {
     const int part = kLpPartBytes / (type == 2 ? 4 : 2);
     return (vocab + part - 1) / part;
 }
+// Whether rows go to a warp each.  1,500 rows of 32 KB take 18.4 us so and 16.3 with a CTA for each, 6,000 rows 49 and 54; one row 11.7 and 5.1.
+// One row of 8 KB takes 4.6 and 5.1, 3,000 of them 8.6 and 34.  A CTA finds its bound among 32 groups, one to a KB: with fewer than `top` of
+// them filled there is none (one row of 8 KB, 20 alternatives: 11.5 us for the warp, 60 for the CTA).
+static bool logprob_by_rows(int rows, int vocab, int type, int top) {
+    const int bytes = vocab * (type == 2 ? 4 : 2);
+    return logprob_parts(vocab, type) == 1 && (rows >= 10 * device_sm_count() || bytes <= 8192 || top > bytes / 1024);
+}
 static bool logprob_shape(int rows, int vocab, int type, int top) {
     return rows >= 1 && rows <= (1 << 23) && vocab >= 1 && vocab <= kLpMaxVocab && type >= 0 && type <= 2 && top >= 0 && top <= kLpMaxTop && top <= vocab;
 }
 
 extern "C" long long ternaspmm_token_logprobs_workspace(int rows, int vocab, int type, int top) {
     if (!logprob_shape(rows, vocab, type, top)) return -1;
-    if (logprob_parts(vocab, type) == 1) return 16;                // (logprob_rows_kernel has none)
+    if (logprob_by_rows(rows, vocab, type, top)) return 16;        // (logprob_rows_kernel has none)
     return (long long)rows * logprob_parts(vocab, type) * (kLpWarps * (int)sizeof(LpSums) + 8 * top);
 }
 
 template <typename T>
 static cudaError_t launch_logprobs(const LogprobParams& p, cudaStream_t stream) {
-    if (p.parts == 1) {
+    if (logprob_by_rows(p.rows, p.vocab, std::is_same<T, float>::value ? 2 : 0, p.top)) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)((p.rows + kLpWarps - 1) / kLpWarps), 1, 1);
         cfg.blockDim = dim3(kLpThreads, 1, 1);
