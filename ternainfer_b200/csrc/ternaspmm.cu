@@ -1313,12 +1313,13 @@ struct Kv4Plan {
     int tiles, row_tiles, cluster, stream;
     bool tcgen05;                          // kv4_prefill_kernel, row_tiles of 128 rows, `cluster` CTAs for each
 };
-static Kv4Plan kv4_plan(int batch, int tokens, int heads, int kv_heads, int max_len) {
+// `keys`: as many as a tile may go over.  (A plan for fewer keys needs no more workspace.)
+static Kv4Plan kv4_plan(int batch, int tokens, int heads, int kv_heads, int keys) {
     const long long rows_all = (long long)tokens * (heads / kv_heads);
     Kv4Plan pl = {rows_all <= 8 ? 1 : 2, 1, 1, 0, false};
     pl.row_tiles = (int)((rows_all + 8 * pl.tiles - 1) / (8 * pl.tiles));
     const int sms = device_sm_count(), slots = (pl.tiles == 1 ? 4 : 2) * sms;
-    const long long items = (long long)batch * kv_heads * pl.row_tiles, blocks = max_len / 32;
+    const long long items = (long long)batch * kv_heads * pl.row_tiles, blocks = (keys + 31) / 32;
     // Several tokens.  The mma.sync kernel goes over the keys once per 16 rows, with a cluster of up to 8 CTAs for each, and the tcgen05 kernel
     // once per 128, in parts.  Up to SMs / 4 tiles of 16 rows the clusters are all resident: 12 tokens of 20 heads over 5, 3,000 keys, 10.8 against 17.5 us
     // (24 tokens: 13.0 against 17.8; 32 tokens, 40 tiles: 8,000 keys, 36 against 21; 128 tokens: 84 against 38).  Below 2 SMs blocks of 32 keys
@@ -1328,15 +1329,17 @@ static Kv4Plan kv4_plan(int batch, int tokens, int heads, int kv_heads, int max_
         pl.row_tiles = (int)((rows_all + kKvpRows - 1) / kKvpRows);
         // Parts of at least 4 tiles of 64 keys, a CTA per SM; two per SM take 1.5 times as long for a tile, so only where a part is longer than 16 tiles:
         // 512 rows of 5 heads, 3,000 keys, 22.7 us with 7 parts and 28.5 with 12; 8 sequences of 128 rows, 30,000 keys, 152 us with 7 and 210 with 3.
-        const long long ctas = (long long)batch * kv_heads * pl.row_tiles, tiles = max_len / kKvpKeys, parts = sms / ctas;
+        const long long ctas = (long long)batch * kv_heads * pl.row_tiles, tiles = keys / kKvpKeys, parts = sms / ctas;
         pl.cluster = (int)std::max(1ll, std::min({tiles > 16 * parts ? 2 * sms / ctas : parts, tiles / 4, 32ll}));
         return pl;
     }
-    if (pl.row_tiles == 1 && items * blocks >= 4ll * kKv4Warps * slots) {
-        pl.stream = slots;
-        return pl;
-    }
-    while (pl.cluster < 8 && pl.cluster * kKv4Warps < blocks && items * pl.cluster < 2 * slots) pl.cluster *= 2;
+    // Clusters as large as all fit beside each other (16 sequences of 700 keys, 5 heads: 9.3 us with 240 CTAs, 14.1 with 640).
+    while (pl.cluster < 8 && pl.cluster * kKv4Warps < blocks && items * pl.cluster * 2 <= slots) pl.cluster *= 2;
+    // One place's share of all keys costs some 10 blocks more than a cluster's: results of two items, the join.  It gains where places stay empty, 17 blocks of
+    // a hundred that they would have had, since those that are taken go faster: 5 heads of 131,000 keys, 40 CTAs, 108 against 36 us; 32 and 64 sequences of
+    // 20,000, 320 CTAs, 122 against 105 and 233 against 188; but 64 of 700, 8 heads, 19 against 43, and 32 of 8,000, 512 CTAs, 61 against 67.
+    const long long ctas = items * pl.cluster, waves = (ctas + slots - 1) / slots;
+    if (pl.row_tiles == 1 && items * blocks >= 4ll * kKv4Warps * slots && 17 * blocks * (waves * slots - ctas) > 1000ll * slots * pl.cluster) pl.stream = slots, pl.cluster = 1;
     return pl;
 }
 // Rows of partial results that a call keeps in its workspace.
@@ -1439,7 +1442,8 @@ extern "C" int ternaspmm_kv4_attend(const __nv_bfloat16* q, const long long* q_s
         (reinterpret_cast<uintptr_t>(out) & 15) || (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15))))
         return t_host_status = ST_BAD_POINTER;
     if (!p.status) return t_host_status = ST_LAUNCH;
-    const Kv4Plan pl = kv4_plan(batch, tokens, heads, kv_heads, max_len);
+    const Kv4Plan pl = kv4_plan(batch, tokens, heads, kv_heads, window ? (int)std::min((long long)max_len, (long long)window + std::min(tokens, kKvpRows)) : max_len);
+    if (kv4_part_rows(batch, kv_heads, pl) * (head_dim + 2) * 4 > workspace_bytes) return t_host_status = ST_BAD_SHAPE;
     p.start = start, p.counts = counts, p.start_stride = start_stride ? 1 : 0, p.out = out, p.tokens = tokens, p.heads = heads, p.window = window;
     p.batch = batch, p.cluster = pl.cluster, p.row_tiles = pl.row_tiles, p.row_bytes = head_dim / 2, p.scale_log2 = scale * 1.4426950408889634f;
     p.part_o = static_cast<float*>(workspace);
