@@ -11,7 +11,13 @@
 // product with its scale.  The order of dimensions within 8 of keys and queries is the one in which codes come out of their words.
 // O stays in tensor memory; it is rescaled only where a row's maximum has left its reference by 2^8.
 // A product takes P = 0 times a value for keys that a row does not see.  So values that are not finite as fp16 (a NaN or infinite scale, or more than
-// 65504) are left out, and the rows that see one of them, or a later one, get NaN in that group of dimensions at the end.
+// 65504) are left out, and the rows that see one of them get NaN in that group of dimensions at the end.
+// Where there are few tiles of rows the keys are cut into parts (`cluster` CTAs to a tile, kv4_prefill_join_kernel).
+//
+// 2,048 tokens of 20 heads over 5 after 2,048: 144 us for 64 GFLOP, 447 TFLOP/s; the floor of the products is 38 us.  A tile of 64 keys takes two CTAs of an
+// SM 3,500 cycles: a softmax warp works through them all (600 to load the scores, 300 for the maximum, 1,750 for exponentials, sums and packing, beside the
+// other CTA's), and so does the thread that issues (1,600 in the queue of MMAs and commits, 1,000 waiting for probabilities).  Without the expansion
+// of keys and values - wrong results - it took 115 us, without exponentials as well 113: no single part is the bound.
 #pragma once
 #include "kv4_attn.cuh"
 

@@ -9,6 +9,9 @@
 // is ever rescaled.  For the alternatives a CTA takes up to eight parts of a row in turn: the k-th largest of the maxima of 32 groups of 8
 // threads is a bound that at least k elements of the first one reach, and few more do (k = 20: 31 on average); they and what exceeds the bound in the
 // other parts are collected, and ranked by counting.  A second kernel, a warp per row, joins the sums and merges the lists.
+//
+// 1,226 rows of 128,256 bf16: 62 us, 5.1 TB/s of 6.46, bound by the exponentials (two 16-bit logits a lane take two of them) at 24 warps an SM; with 20
+// alternatives 106 us: two to four barriers of the CTA and a ranking per run of parts.  3 rows of fp32 with 5 alternatives 9.4 us, two launches' latencies.
 #pragma once
 #include "rotary.cuh"
 #include "w2_tile.cuh"
@@ -702,7 +705,8 @@ struct LogprobGradParams {
     int rows, vocab;
 };
 
-// d/dx_j = g (delta_jt - p_j) - h p_j (log p_j + H).  A CTA per row and part of it, or 256 / threads rows of one part.
+// d/dx_j = g (delta_jt - p_j) - h p_j (log p_j + H).  A CTA per row and part of it, or 256 / threads rows of one part: up
+// to 2,048 tokens a warp (100,000 rows of 300: 64 us against 143).  512 rows of 128,256 fp32 after the forward pass: 149 us together, 5.3 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(256) logprob_grad_kernel(const LogprobGradParams p, int parts, int threads) {
     constexpr int V = 16 / sizeof(T);

@@ -82,7 +82,8 @@ __device__ __forceinline__ void table_values(const float* t, int by_16, float (&
 
 // A thread takes one unit of a token - V pairs of the half layout, V / 2 of the other, or V copied values - in HEADS heads, so that
 // cosines and sines are read once for all of them.  Memory is the bound: what matters is that all loads of a thread are on their way
-// before the first is used, and that the index arithmetic (divisions by multiplication, 32 bits) stays small beside them.
+// before the first is used, and that the index arithmetic (divisions by multiplication, 32 bits) stays small beside them.  Two prompts of 2,048
+// tokens, 64 + 8 heads of 128 in bf16, half layout: 37.7 us, 4.06 TB/s of 6.46 (51 us with a head per thread and divisions); 8 single tokens 1.9 us.
 template <typename T, int V, bool HALF, int HEADS>
 __global__ void __launch_bounds__(256, 4) rotate_kernel(const RotateParams p, uint32_t items) {
     using VT = Vec<T, V>;

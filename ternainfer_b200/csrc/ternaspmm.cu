@@ -641,6 +641,8 @@ extern "C" void ternaspmm_linear_segments(int8_t* x, uint64_t* bitmap, int* tile
 // The tcgen05 kernels release the next launch before they allocate tensor memory, and tcgen05.alloc waits without a limit.  So the CTAs
 // that shared memory lets onto one SM must never ask for more columns than it has: a later launch that took them first would wait for
 // an earlier one that waits for the columns.
+// (kv4_prefill_kernel is not among them: it is launched in plain stream order and releases nothing early, so the CTAs beside it are its own, two with 256
+// columns each, or another stream's, which hold all of theirs and end.)
 struct TmemUse { int smem, columns; };
 constexpr TmemUse kTmemUse[] = {{LargeMSmem<64>::total, 2 * 64}, {LargeMSmem<128>::total, 2 * 128}, {LargeMSmem<256>::total, 2 * 256},
                                 {LargeMSmem<128, true>::total, 2 * 128}, {LargeMSmem<256, true>::total, 2 * 256}, {PairSmem::total, 2 * kPairNT},

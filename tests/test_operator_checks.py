@@ -98,10 +98,12 @@ def test_logprob_statuses(lib):
     good = dict(x=P, ld=10, type=0, t=P, rows=1, vocab=10, top=2, lp=P, h=P, lse=P, tl=P, tt=P, ws=P, bytes=1 << 30)
     for status, change in ((1, dict(rows=0)), (1, dict(vocab=0)), (1, dict(ld=9)), (1, dict(type=-1)), (1, dict(top=33, vocab=50, ld=50)), (1, dict(top=11)), (1, dict(top=-1)),
                            (1, dict(vocab=(1 << 19) + 1, ld=1 << 21)),
-                           (1, dict(bytes=143)), (2, dict(x=None)), (2, dict(x=P + 1)), (2, dict(t=None)), (2, dict(lse=None)), (2, dict(tt=None)), (2, dict(ws=None)),
+                           (1, dict(bytes=15)), (1, dict(vocab=20000, ld=20000, bytes=287)), (2, dict(x=None)), (2, dict(x=P + 1)), (2, dict(t=None)), (2, dict(lse=None)), (2, dict(tt=None)), (2, dict(ws=None)),
                            (2, dict(ws=P + 8))):
         assert lib.ternaspmm_token_logprobs(*{**good, **change}.values(), None) == status, change
-    assert lib.ternaspmm_token_logprobs_workspace(1, 10, 0, 2) == 144 and lib.ternaspmm_token_logprobs_workspace(1, 10, 0, 11) == -1
+    # short rows need next to nothing, longer ones the sums of eight warps and two alternatives for each 32 KB
+    assert lib.ternaspmm_token_logprobs_workspace(1, 10, 0, 2) == 16 and lib.ternaspmm_token_logprobs_workspace(1, 20000, 0, 2) == 288
+    assert lib.ternaspmm_token_logprobs_workspace(1, 10, 0, 11) == -1
     grad = dict(x=P, ld=10, type=2, t=P, rows=1, vocab=10, lse=P, h=P, gl=None, gh=P, out=P)
     for status, change in ((1, dict(rows=0)), (1, dict(ld=9)), (2, dict(out=P + 2)), (2, dict(h=None))):
         assert lib.ternaspmm_token_logprobs_grad(*{**grad, **change}.values(), None) == status, change
