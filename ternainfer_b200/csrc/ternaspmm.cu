@@ -1165,6 +1165,13 @@ extern "C" void ternaspmm_bf16_to_f32(__nv_bfloat16* x, float* y, long long n, c
     checkLastCudaError(__LINE__);
 }
 
+// The status of an entry that returns one: a failed launch is the caller's to handle, and not the next call's error.
+static int launch_result(cudaError_t e) {
+    if (e == cudaSuccess) return t_host_status;
+    cudaGetLastError();
+    return t_host_status = ST_LAUNCH;
+}
+
 // ---- rotary positions (rotary.cuh) ------------------------------------------------------------------
 template <typename T, int V, bool HALF, int HEADS>
 static cudaError_t launch_rotate_heads(RotateParams p, long long tokens_all, cudaStream_t stream) {
@@ -1226,9 +1233,7 @@ extern "C" int ternaspmm_rotate(const void* q, const long long* q_strides, int q
     const cudaError_t e = type == 0 ? launch_rotate_type<__nv_bfloat16>(p, all, half_layout != 0, stream)
                           : type == 1 ? launch_rotate_type<__half>(p, all, half_layout != 0, stream) : launch_rotate_type<float>(p, all, half_layout != 0, stream);
     if (e == cudaErrorMisalignedAddress) return t_host_status = ST_BAD_POINTER;
-    if (e != cudaSuccess) t_host_status = ST_LAUNCH;
-    checkLastCudaError(__LINE__);
-    return t_host_status;
+    return launch_result(e);
 }
 
 // ---- key / value cache in 4 bits (kv4.cuh, kv4_attn.cuh) ----------------------------------------------
@@ -1279,10 +1284,8 @@ extern "C" int ternaspmm_kv4_append(void* k_codes, void* k_scales, void* v_codes
     cfg.gridDim = dim3((unsigned)((items + 255) / 256), 1, 1);
     cfg.blockDim = dim3(256, 1, 1);
     cfg.stream = stream;
-    if (cudaLaunchKernelEx(&cfg, head_dim == 128 ? (here == 1 ? kv4_append_kernel<128, 1> : kv4_append_kernel<128, 2>)
-                                                  : (here == 1 ? kv4_append_kernel<64, 1> : kv4_append_kernel<64, 2>), p, (uint32_t)items) != cudaSuccess) t_host_status = ST_LAUNCH;
-    checkLastCudaError(__LINE__);
-    return t_host_status;
+    return launch_result(cudaLaunchKernelEx(&cfg, head_dim == 128 ? (here == 1 ? kv4_append_kernel<128, 1> : kv4_append_kernel<128, 2>)
+                                                  : (here == 1 ? kv4_append_kernel<64, 1> : kv4_append_kernel<64, 2>), p, (uint32_t)items));
 }
 
 extern "C" int ternaspmm_kv4_read(void* k_codes, void* k_scales, void* v_codes, void* v_scales, int max_len, const long long* start, int start_stride,
@@ -1304,9 +1307,7 @@ extern "C" int ternaspmm_kv4_read(void* k_codes, void* k_scales, void* v_codes, 
     cfg.gridDim = dim3((unsigned)((items + 255) / 256), 1, 1);
     cfg.blockDim = dim3(256, 1, 1);
     cfg.stream = stream;
-    if (cudaLaunchKernelEx(&cfg, head_dim == 128 ? kv4_read_kernel<128> : kv4_read_kernel<64>, p, (uint32_t)items) != cudaSuccess) t_host_status = ST_LAUNCH;
-    checkLastCudaError(__LINE__);
-    return t_host_status;
+    return launch_result(cudaLaunchKernelEx(&cfg, head_dim == 128 ? kv4_read_kernel<128> : kv4_read_kernel<64>, p, (uint32_t)items));
 }
 
 // How an attention call is cut: tiles of 8 query rows per CTA, CTAs for the rows of a key / value head, and CTAs of a cluster for
@@ -1453,9 +1454,7 @@ extern "C" int ternaspmm_kv4_attend(const __nv_bfloat16* q, const long long* q_s
     const cudaError_t e = pl.tcgen05 ? (head_dim == 128 ? launch_kv4_prefill<128>(p, stream) : launch_kv4_prefill<64>(p, stream))
                           : head_dim == 128 ? (pl.tiles == 1 ? launch_kv4_attend<128, 1>(p, pl.stream, stream) : launch_kv4_attend<128, 2>(p, pl.stream, stream))
                                           : (pl.tiles == 1 ? launch_kv4_attend<64, 1>(p, pl.stream, stream) : launch_kv4_attend<64, 2>(p, pl.stream, stream));
-    if (e != cudaSuccess) t_host_status = ST_LAUNCH;
-    checkLastCudaError(__LINE__);
-    return t_host_status;
+    return launch_result(e);
 }
 
 // ---- log probabilities of given tokens (logprobs.cuh) -------------------------------------------------
@@ -1534,10 +1533,7 @@ extern "C" int ternaspmm_token_logprobs(const void* logits, long long ld, int ty
         reinterpret_cast<uintptr_t>(logits) % (type == 2 ? 4 : 2) || (reinterpret_cast<uintptr_t>(workspace) & 15))
         return t_host_status = ST_BAD_POINTER;
     if (!p.status) return t_host_status = ST_LAUNCH;
-    if ((type == 0 ? launch_logprobs<__nv_bfloat16>(p, stream) : type == 1 ? launch_logprobs<__half>(p, stream) : launch_logprobs<float>(p, stream)) != cudaSuccess)
-        t_host_status = ST_LAUNCH;
-    checkLastCudaError(__LINE__);
-    return t_host_status;
+    return launch_result(type == 0 ? launch_logprobs<__nv_bfloat16>(p, stream) : type == 1 ? launch_logprobs<__half>(p, stream) : launch_logprobs<float>(p, stream));
 }
 
 extern "C" int ternaspmm_token_logprobs_grad(const void* logits, long long ld, int type, const long long* targets, int rows, int vocab,
@@ -1555,10 +1551,7 @@ extern "C" int ternaspmm_token_logprobs_grad(const void* logits, long long ld, i
     cfg.gridDim = dim3((unsigned)ctas, 1, 1);
     cfg.blockDim = dim3(256, 1, 1);
     cfg.stream = stream;
-    if (cudaLaunchKernelEx(&cfg, type == 0 ? logprob_grad_kernel<__nv_bfloat16> : type == 1 ? logprob_grad_kernel<__half> : logprob_grad_kernel<float>, p, parts, threads) != cudaSuccess)
-        t_host_status = ST_LAUNCH;
-    checkLastCudaError(__LINE__);
-    return t_host_status;
+    return launch_result(cudaLaunchKernelEx(&cfg, type == 0 ? logprob_grad_kernel<__nv_bfloat16> : type == 1 ? logprob_grad_kernel<__half> : logprob_grad_kernel<float>, p, parts, threads));
 }
 
 extern "C" void ternaspmm_partial_f32(int8_t* x, uint64_t* bitmap, int* tile_offsets, uint16_t* quarter_offsets,

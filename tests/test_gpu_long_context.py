@@ -145,3 +145,44 @@ def test_command(lib, capsys, monkeypatch):
     monkeypatch.setattr(sys, "argv", "generate --layers 1 --prompt_length 20 --gen_length 5 --kv_bits 4 --rope_layout half --rope_linear 4 --top_logprobs 2 --fused_glue".split())
     generate.main()
     assert "log probability per generated token -" in capsys.readouterr().out
+
+
+FAILED_LAUNCH = """
+import torch
+from ternainfer_b200.kv4 import KV4Cache, kv4_append, kv4_attend, kv4_read
+from ternainfer_b200.rotary import rotary_table, rotate
+from ternainfer_b200.scores import token_logprobs
+x = torch.randn((1, 2, 4, 64), device="cuda").bfloat16()
+table, pos, start = rotary_table(64, 64), torch.arange(2, device="cuda"), torch.zeros(1, dtype=torch.int64, device="cuda")
+cache = KV4Cache.empty(1, 4, 64, 64)
+logits, targets = torch.randn((2, 50), device="cuda"), torch.zeros(2, dtype=torch.int64, device="cuda")
+calls = (lambda: rotate(x, x, table, pos), lambda: kv4_append(cache, x, x, start, q=x, table=table), lambda: kv4_read(cache, start, 2),
+         lambda: kv4_attend(x, cache, start), lambda: token_logprobs(logits, targets, 3))
+want = [f() for f in calls]
+torch.cuda.synchronize()
+stream = torch.cuda.Stream()
+try:
+    with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=stream):
+        try:
+            stream.synchronize()                # not allowed: nothing can be launched into this capture any more
+        except RuntimeError:
+            pass
+        for f in calls:
+            try:
+                f()
+            except RuntimeError:
+                print("refused")
+except RuntimeError:
+    print("capture over")
+torch.cuda.synchronize()
+flat = lambda r: [t for t in (r if isinstance(r, tuple) else (r,)) if t is not None]
+print("the same", all(torch.equal(a, b) for f, w in zip(calls, want) for a, b in zip(flat(f()), flat(w))))
+"""
+
+
+def test_a_launch_that_fails_is_an_error_of_the_call():
+    import subprocess
+    import sys
+    from pathlib import Path
+    r = subprocess.run([sys.executable, "-c", FAILED_LAUNCH], capture_output=True, text=True, timeout=300, cwd=Path(__file__).resolve().parents[1])
+    assert r.returncode == 0 and r.stdout.split("\n")[:7] == ["refused"] * 5 + ["capture over", "the same True"], r.stdout + r.stderr
