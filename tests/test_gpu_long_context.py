@@ -186,3 +186,44 @@ def test_a_launch_that_fails_is_an_error_of_the_call():
     from pathlib import Path
     r = subprocess.run([sys.executable, "-c", FAILED_LAUNCH], capture_output=True, text=True, timeout=300, cwd=Path(__file__).resolve().parents[1])
     assert r.returncode == 0 and r.stdout.split("\n")[:7] == ["refused"] * 5 + ["capture over", "the same True"], r.stdout + r.stderr
+
+
+CAPTURED_GRADIENT = """
+import sys
+import torch
+from ternainfer_b200.rotary import rotary_table, rotate
+from ternainfer_b200.scores import token_logprobs
+table, pos, t = rotary_table(64, 64), torch.arange(8, device="cuda"), torch.zeros(8, dtype=torch.int64, device="cuda")
+for shape, call in (((1, 8, 4, 64), lambda x: rotate(x, None, table, pos)[0]), ((8, 500), lambda x: token_logprobs(x, t)[0])):
+    x = torch.randn(shape, device="cuda", requires_grad=True)
+    w = torch.randn_like(call(x))
+    want, = torch.autograd.grad(call(x), x, w)
+    x.grad = torch.zeros_like(x)
+    torch.cuda.synchronize()
+    kept = call(x) if sys.argv[1] == "kept" else None
+    g = torch.cuda.CUDAGraph()
+    try:
+        with torch.cuda.graph(g):
+            call(x).backward(w)
+        x.grad.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        print("replayed", torch.equal(x.grad, want))
+    except RuntimeError:
+        print("refused")
+    if kept is not None:
+        x.grad = None
+        kept.backward(w)
+        print("eager", torch.equal(x.grad, want))
+        break
+"""
+
+
+@pytest.mark.parametrize("which,said", [("none", ["replayed True", "replayed True"]), ("kept", ["refused", "eager True"])])
+def test_captured_gradients(which, said):
+    """A backward pass in a graph; with an eager graph of the same leaf alive torch lets none be captured, which ends neither the process nor that one."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    r = subprocess.run([sys.executable, "-c", CAPTURED_GRADIENT, which], capture_output=True, text=True, timeout=300, cwd=Path(__file__).resolve().parents[1])
+    assert r.returncode == 0 and r.stdout.split("\n")[:-1] == said, r.stdout + r.stderr
