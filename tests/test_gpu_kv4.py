@@ -382,6 +382,28 @@ def test_two_graphs_of_many_tokens(lib):
         assert torch.equal(o, check(x, cache, k, v, s))
 
 
+def test_offsets_beyond_32_bits(lib):
+    """A cache of 6 GB a side: the last tokens of the last sequence, through every entry."""
+    B, H, K, D, L = 40, 16, 8, 128, 262144
+    big = KV4Cache.empty(B, K, L, D)
+    assert big.k_codes.numel() > 1 << 32
+    g = gen(20)
+    k, v = (torch.randn((1, 128, K, D), generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    at = torch.full((B,), L - 128, device="cuda")
+    counts = torch.zeros(B, dtype=torch.int64, device="cuda")
+    counts[-1] = 128
+    kv4_append(big, k.expand(B, -1, -1, -1), v.expand(B, -1, -1, -1), at, counts)
+    got_k, got_v = kv4_read(big, at, 128, counts)
+    lk, lv = levels(k)[0], levels(v)[0]
+    assert torch.equal(got_k[-1:], lk.to(torch.bfloat16)) and torch.equal(got_v[-1:], lv.to(torch.bfloat16)) and not got_k[:-1].any()
+    for T in (1, 3, 40):                  # (no other sequence has values there; a window keeps to what was written)
+        q = torch.randn((B, T, H, D), generator=g, device="cuda").to(torch.bfloat16)
+        out = kv4_attend(q, big, torch.full((B,), L - T, device="cuda"), window=60)
+        want, tol = attention(q[-1:], lk, lv, torch.tensor([128 - T], device="cuda"), torch.tensor([T], device="cuda"), 60, D ** -0.5)
+        assert ((out[-1:].double() - want).abs() <= tol).all() and not out[:-1].any()
+    assert lib.ternaspmm_last_status() == 0
+
+
 def test_refusals(lib):
     cache = KV4Cache.empty(2, 2, 64, 64)
     x, start = torch.zeros((2, 3, 2, 64), device="cuda", dtype=torch.bfloat16), torch.zeros(2, dtype=torch.int64, device="cuda")

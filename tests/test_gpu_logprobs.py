@@ -244,6 +244,26 @@ def test_streams_and_graphs(lib):
     assert all(torch.equal(a, b) for a, b in zip(out, token_logprobs(x, t, 5)))
 
 
+@pytest.mark.parametrize("N,V", [(17000, 128256), (1100000, 2000)])
+def test_offsets_beyond_32_bits(lib, N, V):
+    """More than 2^31 logits: the last rows give what they give alone, the gradient included."""
+    x = torch.empty((N, V), device="cuda", dtype=torch.bfloat16).normal_(generator=gen(1))
+    assert x.numel() > 1 << 31
+    t = torch.randint(0, V, (N,), generator=gen(2), device="cuda")
+    w = torch.randn(N, generator=gen(3), device="cuda")
+    x.requires_grad_()
+    r = token_logprobs(x, t, 4)
+    grad, = torch.autograd.grad(r.logprob, x, w)
+    y = x.detach()[-3:].clone().requires_grad_()
+    alone = check(y.detach(), t[-3:], 4)
+    want, = torch.autograd.grad(token_logprobs(y, t[-3:]).logprob, y, w[-3:])
+    # (another number of rows may be summed in another order: both are within check()'s bound)
+    bound = 2 * ((V / 512 + 40) * 2.0 ** -24 + 2.0 ** -20) + alone.logprob.abs() * 2.0 ** -21
+    assert ((r.logprob[-3:] - alone.logprob).abs() <= bound).all() and torch.equal(r.top_token[-3:], alone.top_token)
+    assert ((grad[-3:].float() - want.float()).abs() <= want.float().abs() * 2.0 ** -7 + w[-3:, None].abs() * 2.0 ** -126).all()
+    assert lib.ternaspmm_last_status() == 0
+
+
 def test_refusals(lib):
     x, t = torch.zeros((2, 50), device="cuda"), torch.zeros(2, dtype=torch.int64, device="cuda")
     for bad in (dict(logits=x.double()), dict(targets=t.int()), dict(targets=t[:1]), dict(targets=t.cpu()), dict(top=33), dict(top=-1), dict(logits=x[:, :0]),
