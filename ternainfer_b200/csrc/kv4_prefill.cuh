@@ -30,7 +30,7 @@ struct KvpSmem {
     static constexpr int q = 0, q_block = kKvpRows * 128, q_bytes = D / 64 * q_block;
     static constexpr int k = q + q_bytes, k_block = kKvpKeys * 128, k_bytes = D / 64 * k_block;   // two stages
     static constexpr int v = k + 2 * k_bytes, v_bytes = D * 128;                                   // two stages: a row per dimension
-    static constexpr int bars = v + 2 * v_bytes;                   // q, k full / empty, v full / empty, s full, p full (2 each), o done
+    static constexpr int bars = v + 2 * v_bytes;                   // q; keys, values, scores, probabilities and O of a tile there (2 each)
     static constexpr int slot = bars + 16 * 8, abort_flag = slot + 4, bad = slot + 16;             // bad: first key of each group that is not finite
     static constexpr int total = 1024 + bad + 32;
     static constexpr uint32_t columns = 256;                       // O: D, S: two buffers of 64
@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
     uint8_t* smem = raw_smem + ((1024 - (smem_u32(raw_smem) & 1023)) & 1023);
     const uint32_t sb = smem_u32(smem);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t b_q = sb + Sm::bars, b_kf = b_q + 8, b_ke = b_kf + 16, b_vf = b_ke + 16, b_ve = b_vf + 16, b_s = b_ve + 16, b_p = b_s + 16, b_o = b_p + 16;
+    const uint32_t b_q = sb + Sm::bars, b_kf = b_q + 8, b_vf = b_kf + 16, b_s = b_vf + 16, b_p = b_s + 16, b_o = b_p + 16;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Sm::abort_flag);
     int* bad = reinterpret_cast<int*>(smem + Sm::bad);
     // the longest rows first
@@ -127,11 +127,9 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
     if (tid == 0) {
         mbar_init(b_q, 4);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(b_kf + 8 * i, 2), mbar_init(b_ke + 8 * i, 1);
-            mbar_init(b_vf + 8 * i, 2), mbar_init(b_ve + 8 * i, 1);
-            mbar_init(b_s + 8 * i, 1), mbar_init(b_p + 8 * i, 4);
+            mbar_init(b_kf + 8 * i, 2), mbar_init(b_vf + 8 * i, 2);
+            mbar_init(b_s + 8 * i, 1), mbar_init(b_p + 8 * i, 4), mbar_init(b_o + 8 * i, 1);
         }
-        mbar_init(b_o, 1);
         mbar_fence_init();
         *abort_flag = 0;
         for (int i = 0; i < G; ++i) bad[i] = 0x7fffffff;
@@ -217,7 +215,7 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
                 }
                 l *= f;
                 if (j > 0) {                                       // O is complete up to tile j - 1 before it is touched
-                    ok = kvp_wait_warp(b_o, (j - 1) & 1, abort_flag);
+                    ok = kvp_wait_warp(b_o + 8 * (buf ^ 1), ((j - 1) >> 1) & 1, abort_flag);
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll 1
@@ -253,7 +251,7 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
             tc_fence_before();
             kvp_arrive(b_p + 8 * buf, lane);
         }
-        if (ok && tiles > 0) ok = kvp_wait_warp(b_o, (tiles - 1) & 1, abort_flag);
+        if (ok && tiles > 0) ok = kvp_wait_warp(b_o + 8 * ((tiles - 1) & 1), ((tiles - 1) >> 1) & 1, abort_flag);
     } else if (warp < 6) {                                         // ---- keys: one per thread
         const int key = tid - 128;
         const uint8_t* kc = p.c.k_codes + (row0 + key) * (D / 2);
@@ -275,7 +273,7 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
 #pragma unroll
             for (int i = 0; i < G / 2; ++i) sc[i] = sc_next[i];
             if (j + 1 < tiles) load(j + 1, w_next, sc_next);
-            if (j >= 2 && !kvp_wait_warp(b_ke + 8 * st, ((j >> 1) - 1) & 1, abort_flag)) break;
+            if (j >= 2 && !kvp_wait_warp(b_s + 8 * st, ((j >> 1) - 1) & 1, abort_flag)) break;
             const uint32_t dst = sb + Sm::k + st * Sm::k_bytes + key * 128;
             // 16 bytes t of a row hold word t of every group (64 dimensions: 8 bytes)
             uint32_t words[4 * G];
@@ -315,7 +313,7 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
 #pragma unroll
                 for (int i = 0; i < G / 2; ++i) w[k][i] = w_next[k][i], sc[k][i] = sc_next[k][i];
             if (j + 1 < tiles) load(j + 1, w_next, sc_next);
-            if (j >= 2 && !kvp_wait_warp(b_ve + 8 * st, ((j >> 1) - 1) & 1, abort_flag)) break;
+            if (j >= 2 && !kvp_wait_warp(b_o + 8 * st, ((j >> 1) - 1) & 1, abort_flag)) break;
             const uint32_t dst = sb + Sm::v + st * Sm::v_bytes;
             // keys behind the last one hold anything; scales beyond 8188 (0x6fff) make values that fp16 does not hold
             uint32_t big = 0;
@@ -364,23 +362,21 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
             for (int i = 0; i < D / 16; ++i)
                 umma_f16(t_s + st * 64, umma_desc_sw128(sb + Sm::q + (i >> 2) * Sm::q_block + (i & 3) * 32),
                          umma_desc_sw128(k + (i >> 2) * Sm::k_block + (i & 3) * 32), id_s, i > 0);
-            umma_commit(b_s + 8 * st);
-            umma_commit(b_ke + 8 * st);
+            umma_commit(b_s + 8 * st);                             // (the scores are there, and the keys' place is free)
             return true;
         };
         if (ok && tiles > 0) ok = scores(0);
         for (int j = 0; ok && j < tiles; ++j) {
             const int st = j & 1;
             // the buffer that the scores of tile j + 1 go to is the one that the product of tile j - 1 with V reads
-            if (j + 1 < tiles) ok = (j == 0 || kvp_wait(b_o, (j - 1) & 1, abort_flag)) && scores(j + 1);
+            if (j + 1 < tiles) ok = (j == 0 || kvp_wait(b_o + 8 * (st ^ 1), ((j - 1) >> 1) & 1, abort_flag)) && scores(j + 1);
             ok = ok && kvp_wait(b_vf + 8 * st, (j >> 1) & 1, abort_flag) && kvp_wait(b_p + 8 * st, (j >> 1) & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
             const uint32_t v = sb + Sm::v + st * Sm::v_bytes;
 #pragma unroll
             for (int i = 0; i < kKvpKeys / 16; ++i) umma_f16_ts(t_o, t_s + st * 64 + i * 8, umma_desc_sw128(v + i * 32), id_o, j > 0 || i > 0);
-            umma_commit(b_ve + 8 * st);
-            umma_commit(b_o);
+            umma_commit(b_o + 8 * st);
         }
     }
     __syncwarp();

@@ -9,7 +9,7 @@ from test_gpu_kv4 import attention, levels
 from ternainfer_b200 import model as model_module
 from ternainfer_b200.convert.convert_TernaInfer import random_checkpoint
 from ternainfer_b200.generate import FastGen, GenArgs
-from ternainfer_b200.kv4 import KV4Cache, kv4_append, kv4_attend
+from ternainfer_b200.kv4 import KV4Cache, kv4_append, kv4_attend, kv4_read
 from ternainfer_b200.model import ModelArgs, Transformer
 from ternainfer_b200.rotary import rotary_table, rotate
 from ternainfer_b200.scores import token_logprobs
@@ -145,6 +145,31 @@ def test_command(lib, capsys, monkeypatch):
     monkeypatch.setattr(sys, "argv", "generate --layers 1 --prompt_length 20 --gen_length 5 --kv_bits 4 --rope_layout half --rope_linear 4 --top_logprobs 2 --fused_glue".split())
     generate.main()
     assert "log probability per generated token -" in capsys.readouterr().out
+
+
+def test_empty_calls(lib):
+    """No rows, no tokens, no sequences; a single row without leading dimensions; transposed, sliced and broadcast logits."""
+    for lead in ((0,), (2, 0), ()):
+        x, t = torch.randn(*lead, 50, device="cuda", requires_grad=True), torch.zeros(lead, dtype=torch.int64, device="cuda")
+        r = token_logprobs(x, t, 3)
+        assert r.logprob.shape == lead and r.top_token.shape == (*lead, 3)
+        assert torch.autograd.grad(r.logprob.sum() + r.entropy.sum(), x)[0].shape == x.shape
+    cache, start = KV4Cache.empty(2, 2, 64, 64), torch.zeros(2, dtype=torch.int64, device="cuda")
+    none = torch.randn(2, 0, 2, 64, device="cuda").bfloat16()
+    assert kv4_append(cache, none, none, start) is None and kv4_attend(none, cache, start).shape == none.shape
+    assert all(t.shape == none.shape for t in kv4_read(cache, start, 0))
+    for shape in ((0, 3, 2, 64), (2, 0, 2, 64)):
+        q = torch.randn(shape, device="cuda", requires_grad=True)
+        a, b = rotate(q, q.detach(), rotary_table(64, 64), torch.zeros(shape[1], dtype=torch.int64, device="cuda"))
+        assert a.shape == b.shape == torch.autograd.grad(a.sum(), q)[0].shape == shape
+    t = torch.zeros(8, dtype=torch.int64, device="cuda")
+    for x in (torch.randn(50, 8, device="cuda").t(), torch.randn(8, 101, device="cuda")[:, 1:51], torch.randn(50, device="cuda").expand(8, 50)):
+        x.requires_grad_()
+        y = token_logprobs(x, t)
+        want = torch.log_softmax(x.double(), -1)[:, 0]
+        assert ((y.logprob.double() - want).abs() <= 2.0 ** -19 + want.abs() * 2.0 ** -22).all()
+        assert torch.autograd.grad(y.logprob.sum(), x)[0].shape == x.shape
+    assert lib.ternaspmm_last_status() == 0
 
 
 FAILED_LAUNCH = """
