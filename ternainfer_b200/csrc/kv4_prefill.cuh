@@ -14,7 +14,7 @@
 // 65504) are left out, and the rows that see one of them get NaN in that group of dimensions at the end.
 // Where there are few tiles of rows the keys are cut into parts (`cluster` CTAs to a tile, kv4_prefill_join_kernel).
 //
-// 2,048 tokens of 20 heads over 5 after 2,048: 144 us for 64 GFLOP, 447 TFLOP/s; the floor of the products is 38 us.  A tile of 64 keys takes two CTAs of an
+// 2,048 tokens of 20 heads over 5 after 2,048: 140 us for 64 GFLOP, 460 TFLOP/s; the floor of the products is 38 us.  A tile of 64 keys takes two CTAs of an
 // SM 3,500 cycles: a softmax warp works through them all (600 to load the scores, 300 for the maximum, 1,750 for exponentials, sums and packing, beside the
 // other CTA's), and so does the thread that issues (1,600 in the queue of MMAs and commits, 1,000 waiting for probabilities).  Without the expansion
 // of keys and values - wrong results - it took 115 us, without exponentials as well 113: no single part is the bound.
@@ -256,23 +256,18 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
         const int key = tid - 128;
         const uint8_t* kc = p.c.k_codes + (row0 + key) * (D / 2);
         const __half* ks = p.c.k_scales + (row0 + key) * G;
-        uint4 w[D / 32], w_next[D / 32];                           // (the next tile is on its way while one is expanded)
-        uint32_t sc[G / 2], sc_next[G / 2];
+        uint4 w[D / 32];
+        uint32_t sc[G / 2];
         auto load = [&](int j, uint4 (&w)[D / 32], uint32_t (&sc)[G / 2]) {
             const uint8_t* src = kc + (size_t)j * kKvpKeys * (D / 2);
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) w[i] = ldg_128(src + 16 * i);
             ldg_words(ks + (size_t)j * kKvpKeys * G, sc);
         };
-        if (tiles > 0) load(0, w_next, sc_next);
+        if (tiles > 0) load(0, w, sc);
 #pragma unroll 1
         for (int j = 0; j < tiles; ++j) {
             const int st = j & 1;
-#pragma unroll
-            for (int i = 0; i < D / 32; ++i) w[i] = w_next[i];
-#pragma unroll
-            for (int i = 0; i < G / 2; ++i) sc[i] = sc_next[i];
-            if (j + 1 < tiles) load(j + 1, w_next, sc_next);
             if (j >= 2 && !kvp_wait_warp(b_s + 8 * st, ((j >> 1) - 1) & 1, abort_flag)) break;
             const uint32_t dst = sb + Sm::k + st * Sm::k_bytes + key * 128;
             // 16 bytes t of a row hold word t of every group (64 dimensions: 8 bytes)
@@ -291,12 +286,13 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
             }
             fence_proxy_async_smem();
             kvp_arrive(b_kf + 8 * st, lane);
+            if (j + 1 < tiles) load(j + 1, w, sc);                 // (arrives while the place for it is waited for)
         }
     } else if (warp < 8) {                                         // ---- values: 16 dimensions of 8 keys per thread
         const int oct = tid & 7, g = (tid - 192) >> 3;             // keys 8 oct .. + 7, halfword g of every group
         const uint8_t* vc = p.c.v_codes + (row0 + 8 * oct) * (D / 2) + g * (G * 2);
         const __half* vs = p.c.v_scales + (row0 + 8 * oct) * G;
-        uint32_t w[8][G / 2], sc[8][G / 2], w_next[8][G / 2], sc_next[8][G / 2];
+        uint32_t w[8][G / 2], sc[8][G / 2];
         auto load = [&](int j, uint32_t (&w)[8][G / 2], uint32_t (&sc)[8][G / 2]) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
@@ -304,15 +300,10 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
                 ldg_words(vs + ((size_t)j * kKvpKeys + k) * G, sc[k]);
             }
         };
-        if (tiles > 0) load(0, w_next, sc_next);
+        if (tiles > 0) load(0, w, sc);
 #pragma unroll 1
         for (int j = 0; j < tiles; ++j) {
             const int st = j & 1, key0 = base + j * kKvpKeys + 8 * oct;
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-#pragma unroll
-                for (int i = 0; i < G / 2; ++i) w[k][i] = w_next[k][i], sc[k][i] = sc_next[k][i];
-            if (j + 1 < tiles) load(j + 1, w_next, sc_next);
             if (j >= 2 && !kvp_wait_warp(b_o + 8 * st, ((j >> 1) - 1) & 1, abort_flag)) break;
             const uint32_t dst = sb + Sm::v + st * Sm::v_bytes;
             // keys behind the last one hold anything; scales beyond 8188 (0x6fff) make values that fp16 does not hold
@@ -348,6 +339,7 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
             }
             fence_proxy_async_smem();
             kvp_arrive(b_vf + 8 * st, lane);
+            if (j + 1 < tiles) load(j + 1, w, sc);                 // (arrives while the place for it is waited for)
         }
     } else if (lane == 0) {                                        // ---- products
         const uint32_t id_s = (1u << 4) | ((uint32_t)(kKvpKeys >> 3) << 17) | ((uint32_t)(kKvpRows >> 4) << 24);
