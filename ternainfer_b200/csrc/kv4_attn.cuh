@@ -208,10 +208,11 @@ __global__ void __launch_bounds__(kKv4Warps * 32, NT == 1 ? 4 : 2) kv4_attn_kern
         long long at = all * blockIdx.x / gridDim.x;
         left = all * (blockIdx.x + 1) / gridDim.x - at;
         if (left == 0) return;
-        // the sequence, head and block where this CTA's part begins
-        int* found = reinterpret_cast<int*>(ml);
+        // the sequence, head and block where this CTA's part begins: every warp finds them, by shuffles (shared memory that carried them from one
+        // warp to the others would have to outlive their reading, and all of it belongs to the rings and the query's fragments from here on)
+        b = hk = begin = 0;
         long long before = 0;
-        for (int b0 = 0; b0 < p.batch; b0 += 32) {                 // (every warp the same)
+        for (int b0 = 0; b0 < p.batch; b0 += 32) {
             const int n = b0 + lane < p.batch ? blocks_of(b0 + lane) : 0;
             long long upto = (long long)n * p.c.kv_heads;
 #pragma unroll
@@ -221,16 +222,14 @@ __global__ void __launch_bounds__(kKv4Warps * 32, NT == 1 ? 4 : 2) kv4_attn_kern
             }
             const unsigned has = __ballot_sync(0xffffffffu, before + upto > at);
             if (has) {
-                if (warp == 0 && lane == __ffs(has) - 1) {
-                    const long long in = at - (before + upto - (long long)n * p.c.kv_heads);
-                    found[0] = b0 + lane, found[1] = (int)(in / n), found[2] = (int)(in % n);
-                }
+                const int src = __ffs(has) - 1, blocks = __shfl_sync(0xffffffffu, n, src);
+                const long long in = at - (before + __shfl_sync(0xffffffffu, upto, src) - (long long)blocks * p.c.kv_heads);
+                b = b0 + src, hk = (int)(in / blocks), begin = (int)(in % blocks);
                 break;
             }
             before += __shfl_sync(0xffffffffu, upto, 31);
         }
-        __syncthreads();
-        b = found[0], hk = found[1], begin = found[2];
+        __syncthreads();                                           // (the query's fragments come where kv4_cta_sum's parts are)
     }
 #pragma unroll 1
     for (bool first_part = true;; first_part = false) {

@@ -1,0 +1,27 @@
+"""GPU: calls of the rotary, 4-bit cache and scoring operators at their edges, each against its definition in 64 bits or against torch's own manner."""
+import pytest
+import torch
+
+from test_gpu_kv4 import check as check_attention, levels
+from test_gpu_logprobs import gen
+from ternainfer_b200.kv4 import KV4Cache, kv4_append, kv4_attend
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("D,H,K", [(64, 8, 2), (128, 12, 1)])
+def test_equal_shares_of_short_sequences_in_a_large_cache(lib, D, H, K):
+    """So many places that keys are cut into equal shares whatever the lengths: each CTA finds its first sequence, head and block before it writes
+    the query's fragments; again and again the same numbers."""
+    B, L, n = 400 // K, 6016, 700
+    cache = KV4Cache.empty(B, K, L, D)
+    k, v = (torch.randn((B, n, K, D), generator=gen(i), device="cuda").to(torch.bfloat16) for i in (1, 2))
+    kv4_append(cache, k, v, torch.zeros(1, dtype=torch.int64, device="cuda"))
+    k, v = levels(k)[0], levels(v)[0]
+    q = torch.randn((B, 1, H, D), generator=gen(3), device="cuda").to(torch.bfloat16)
+    for low, high in ((0, n), (n - 3, n), (0, 2)):
+        start = torch.randint(low, high, (B,), generator=gen(high), device="cuda")
+        got = check_attention(q, cache, k, v, start)
+        for _ in range(30):
+            assert torch.equal(kv4_attend(q, cache, start), got)
+    assert lib.ternaspmm_last_status() == 0
