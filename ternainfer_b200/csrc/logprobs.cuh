@@ -498,6 +498,7 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) logprob_rows_kernel(
     if (r >= (unsigned)p.rows) return;                             // (no barrier of the CTA below)
     unsigned long long* cand = lists[warp];
     LpPart<T> at(p, r, 0);
+    at.parts = max(1, (at.vecs + 32 * kLpVecs - 1) / (32 * kLpVecs));   // pieces of 4 KB: the row's last elements go with the last one, as ids ascend
     const long long target = p.targets[r];
     const float xt = target >= 0 && target < p.vocab ? Elem<T>::get(at.row[target]) : 0.f;
     if (lane == 0) counts[warp] = 0;
@@ -505,8 +506,8 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) logprob_rows_kernel(
     uint32_t bound = 0;
     bool full = false;
 #pragma unroll 1
-    for (int k = 0; k == 0 || at.first < at.vecs; ++k, at.first += 32 * kLpVecs) {
-        const int edge = k == 0 ? at.edge(lane) : -1, n = min(kLpVecs, (at.vecs - at.first + 31) / 32);
+    for (int k = 0; k < at.parts; ++k, ++at.part, at.first += 32 * kLpVecs) {
+        const int edge = at.edge(lane), n = min(kLpVecs, (at.vecs - at.first + 31) / 32);
         auto again = [&](int j) { return at.has(j, lane) ? Vec16{ldg_128(at.row + at.index(j, lane))} : Vec16{make_uint4(Vec16::none, Vec16::none, Vec16::none, Vec16::none)}; };
         Vec16 x16[kLpVecs];
 #pragma unroll
@@ -571,7 +572,7 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) logprob_rows_kernel(
             for (int i = 0; i < V; ++i)
                 if (!(x[i] < bf)) push(x[i], at.index(j, lane) + i);
         }
-        if (edge >= 0) push(xe, edge);
+        if (edge >= 0 && !(bound == 0xffffffffu && k > 0)) push(xe, edge);
         __syncwarp();
         int c = counts[warp];
         if (c > kLpRowCandidates) {                                // many elements at the bound or above it: found at the end

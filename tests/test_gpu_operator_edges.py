@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from test_gpu_kv4 import check as check_attention, levels
-from test_gpu_logprobs import gen
+from test_gpu_logprobs import TYPES, check as check_scores, gen
 from ternainfer_b200.kv4 import KV4Cache, kv4_append, kv4_attend
 
 pytestmark = pytest.mark.gpu
@@ -24,4 +24,24 @@ def test_equal_shares_of_short_sequences_in_a_large_cache(lib, D, H, K):
         got = check_attention(q, cache, k, v, start)
         for _ in range(30):
             assert torch.equal(kv4_attend(q, cache, start), got)
+    assert lib.ternaspmm_last_status() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,size", [(16, 8192), (1500, 20000), (1500, 32000)])
+def test_ties_between_a_rows_end_and_its_middle(lib, dtype, N, size):
+    """Rows of several 4 KB at a warp each that end off a 16-byte boundary: of equal logits the lowest ids, whichever piece of the row they are in."""
+    V = size // torch.finfo(dtype).bits * 8 - 3
+    chunk = 4096 // torch.finfo(dtype).bits * 8
+    base = (0.5 * torch.randn((N, V + 9), generator=gen(V), device="cuda")).clamp(-4, 4).to(dtype)
+    t = torch.randint(0, V, (N,), generator=gen(1), device="cuda")
+    for top in (1, 5, 20, 32):
+        y = base.clone()
+        for off in (0, 1, 6):
+            x = y[:, off: off + V]
+            x[:, V - 1] = 7.0
+            x[:, V - 2] = 6.0
+            x[:, chunk + 100: chunk + 103] = 7.0
+            x[:, 50: 50 + 7 * (top - 1): 7] = 7.0
+            check_scores(x, t, top)
     assert lib.ternaspmm_last_status() == 0
