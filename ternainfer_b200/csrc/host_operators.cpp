@@ -295,15 +295,14 @@ Tensor logit_rows(const Tensor& x) {
 long long row_step(const Tensor& rows) { return std::max<int64_t>(rows.stride(0), rows.size(1)); }
 
 struct Scores {
-    Tensor rows, targets, stats, top_logprob, top_token;
+    Tensor stats, top_logprob, top_token;
 };
 
 Scores scores_launch(const Tensor& logits, const Tensor& targets, int64_t top) {
     const c10::cuda::CUDAGuard guard(logits.device());
     Scores s;
-    s.rows = logit_rows(logits);
-    s.targets = targets.reshape({-1}).contiguous();
-    const int64_t N = s.rows.size(0), V = s.rows.size(1);
+    const Tensor rows = logit_rows(logits), ids = targets.reshape({-1}).contiguous();
+    const int64_t N = rows.size(0), V = rows.size(1);
     TORCH_CHECK_VALUE(N <= INT_MAX && V <= INT_MAX, "logits of ", logits.sizes());
     s.stats = at::empty({4, N}, logits.options().dtype(at::kFloat));
     auto shape = targets.sizes().vec();
@@ -314,7 +313,7 @@ Scores scores_launch(const Tensor& logits, const Tensor& targets, int64_t top) {
         const long long need = ternaspmm_token_logprobs_workspace((int)N, (int)V, type_code(logits), (int)top);
         TORCH_CHECK_VALUE(need >= 0, "token_logprobs: a vocabulary of ", V, " (up to 2^19)");
         const Tensor work = at::empty({need}, logits.options().dtype(at::kByte));   // of this call alone
-        launched(ternaspmm_token_logprobs(ptr(s.rows), row_step(s.rows), type_code(logits), as<long long>(s.targets), (int)N, (int)V, (int)top, stats, stats + N,
+        launched(ternaspmm_token_logprobs(ptr(rows), row_step(rows), type_code(logits), as<long long>(ids), (int)N, (int)V, (int)top, stats, stats + N,
                                           stats + 2 * N, top ? as<float>(s.top_logprob) : nullptr, top ? as<long long>(s.top_token) : nullptr, ptr(work), need,
                                           c10::cuda::getCurrentCUDAStream().stream()),
                  "ternaspmm_token_logprobs");
@@ -330,7 +329,8 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
         const auto shape = targets.sizes();
         // (results of their own: a program may write to them before the backward pass)
         variable_list out = {s.stats[0].reshape(shape).clone(), s.stats[1].reshape(shape).clone()};
-        ctx->save_for_backward({logits, s.targets, s.stats});
+        // (the caller's own targets: a view made here would not share the counter by which torch notices that they have changed since)
+        ctx->save_for_backward({logits, targets, s.stats});
         if (top) {
             out.push_back(s.top_logprob), out.push_back(s.top_token);
             ctx->mark_non_differentiable({s.top_logprob, s.top_token});
@@ -344,7 +344,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
         const auto saved = ctx->get_saved_variables();
         const Tensor &logits = saved[0], &stats = saved[2];
         const c10::cuda::CUDAGuard guard(logits.device());
-        const Tensor rows = logit_rows(logits);
+        const Tensor rows = logit_rows(logits), ids = saved[1].reshape({-1}).contiguous();
         const int64_t N = rows.size(0), V = rows.size(1);
         const Tensor grad = at::empty({N, V}, rows.options());
         OptTensor g[2];
@@ -352,7 +352,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
             if (grads[i].defined()) g[i] = grads[i].contiguous();
         float* s = as<float>(stats);
         if (N)
-            launched(ternaspmm_token_logprobs_grad(ptr(rows), row_step(rows), type_code(rows), as<long long>(saved[1]), (int)N, (int)V, s + 2 * N, s + N, as<float>(g[0]),
+            launched(ternaspmm_token_logprobs_grad(ptr(rows), row_step(rows), type_code(rows), as<long long>(ids), (int)N, (int)V, s + 2 * N, s + N, as<float>(g[0]),
                                                    as<float>(g[1]), ptr(grad), c10::cuda::getCurrentCUDAStream().stream()),
                      "ternaspmm_token_logprobs_grad");
         out[0] = grad.reshape(logits.sizes());

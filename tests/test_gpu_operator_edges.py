@@ -5,6 +5,7 @@ import torch
 from test_gpu_kv4 import check as check_attention, levels
 from test_gpu_logprobs import TYPES, check as check_scores, gen
 from ternainfer_b200.kv4 import KV4Cache, kv4_append, kv4_attend
+from ternainfer_b200.scores import token_logprobs
 
 pytestmark = pytest.mark.gpu
 
@@ -45,3 +46,15 @@ def test_ties_between_a_rows_end_and_its_middle(lib, dtype, N, size):
             x[:, 50: 50 + 7 * (top - 1): 7] = 7.0
             check_scores(x, t, top)
     assert lib.ternaspmm_last_status() == 0
+
+
+def test_targets_that_change_before_the_backward_pass(lib):
+    """As with torch's own operators: an error, not the gradient of other tokens."""
+    x = torch.randn((4, 6, 500), generator=gen(1), device="cuda", requires_grad=True)
+    for t in (torch.randint(0, 500, (4, 6), generator=gen(2), device="cuda"), torch.randint(0, 500, (4, 12), generator=gen(3), device="cuda")[:, ::2]):
+        want, = torch.autograd.grad(token_logprobs(x, t.clone()).logprob.sum(), x)
+        r = token_logprobs(x, t, 2)
+        assert torch.equal(torch.autograd.grad(r.logprob.sum(), x, retain_graph=True)[0], want)
+        t[0, 0] = 7
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(r.logprob.sum(), x)
