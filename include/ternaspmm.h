@@ -346,7 +346,8 @@ int ternaspmm_rotate(const void* q, const long long* q_strides, int q_heads, voi
  * Codes are packed two a byte, the even one low; a key row then holds 4-byte word t of every group, t = 0 .. 3, a value row 2-byte
  * halfword g of every group, g = 0 .. 7.
  * start: int64 position of the first of `tokens` new tokens, of each sequence (start_stride 1) or of all (0); counts: int64 [batch],
- * how many of them there are (null: all).  Sequences whose tokens do not fit into the cache are refused as a whole.
+ * how many of them there are (null: all).  Sequences whose tokens do not fit into the cache, or (_append with
+ * tables) reach beyond table_len, are refused as a whole: nothing of them is written, the rotated part of their queries is NaN.
  *
  * _append: rotates q (may be null; then no q_out) and k by position where tables are given (bf16 results, ternaspmm_rotate's
  * arithmetic) and writes the rows start .. start + count - 1.  8-byte aligned inputs, strides multiples of 4; results 16-byte aligned.

@@ -82,13 +82,13 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4AppendParams p
     uint32_t hg, t;
     const uint32_t bt = p.head_groups.div(live ? item / U : 0u, hg), b = p.tokens.div(bt, t);
     const long long start = p.start[(long long)b * p.start_stride], count = p.counts ? p.counts[b] : (long long)p.tokens.d;
-    const bool fits = kv4_fits(start, count, (int)p.tokens.d, p.c.max_len);
+    // a sequence is refused as a whole where one of its tokens lies outside of the cache or of the table: not written, its queries NaN
+    const bool fits = kv4_fits(start, count, (int)p.tokens.d, p.c.max_len) && (!p.cos_tab || count == 0 || start + count <= p.table_len);
     if (!fits && live) *p.status = 1;
     const long long pos = start + t;
     const int half = p.rotary / 2;
-    const bool turns = p.cos_tab && e < p.rotary, pos_ok = pos >= 0 && pos < p.table_len;
-    // a padded query behind the table takes NaN, and is nobody's concern
-    if (turns && live && fits && t < count && !pos_ok) *p.status = 1;
+    // (a padded query behind the table takes NaN as well, and is nobody's concern)
+    const bool turns = p.cos_tab && e < p.rotary, pos_ok = fits && pos < p.table_len;
     // pairs of 8 values whose other halves are 8 values too, or neighbours: whole vectors
     const bool whole = p.half ? half % 8 == 0 : p.rotary % 8 == 0, second = p.half && e >= half;
     uint4 x[HEADS], y[HEADS];

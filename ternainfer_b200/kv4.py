@@ -69,7 +69,8 @@ def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, start: torch.T
     """Writes T new tokens of every sequence: keys and values bf16 [B, T, Hkv, D] (strided views as they are) into rows start[b] .. of the
     cache, ``start`` int64 [B] or [1] on the device; of sequence b only the first counts[b], rows behind those stay as they were.  With ``table``
     keys - and queries bf16 [B, T, H, D], whose rotated form is returned - are turned by their positions first, in the same
-    launch.  A sequence that does not fit is not written, and the library's status is 1."""
+    launch.  A sequence that does not fit into the cache, or has a token at a position that the table lacks, is not written at all,
+    its queries come back as NaN, and the library's status is 1."""
     cos, sin, half = (None, None, False) if table is None else (table.cos, table.sin, table.layout == "half")
     return load_host_call().kv4_append(*cache._tensors(), k, v, start, counts, q, cos, sin, half)
 

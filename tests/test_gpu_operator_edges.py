@@ -2,9 +2,10 @@
 import pytest
 import torch
 
-from test_gpu_kv4 import check as check_attention, levels
+from test_gpu_kv4 import check as check_attention, filled, levels
 from test_gpu_logprobs import TYPES, check as check_scores, gen
 from ternainfer_b200.kv4 import KV4Cache, kv4_append, kv4_attend
+from ternainfer_b200.rotary import rotary_table, rotate
 from ternainfer_b200.scores import token_logprobs
 
 pytestmark = pytest.mark.gpu
@@ -58,3 +59,36 @@ def test_targets_that_change_before_the_backward_pass(lib):
         t[0, 0] = 7
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             torch.autograd.grad(r.logprob.sum(), x)
+
+
+@pytest.mark.parametrize("layout,n", [("interleaved", 64), ("half", 64), ("half", 32), ("interleaved", 36), ("half", 36)])
+def test_append_beyond_the_table(lib, layout, n):
+    """A cache longer than the rotary table: a sequence with a token at a position that the table lacks is not written at all, and its queries are NaN."""
+    B, T, K, D, L = 5, 3, 2, 64, 100
+    table = rotary_table(D, L, rotary_dim=n, layout=layout)
+    cache, *_ = filled(B, K, 128, D, 3)
+    before = [t.clone() for t in cache._tensors()]
+    q, k, v = torch.randn((B, T, 4 + 2 * K, D), generator=gen(4), device="cuda").to(torch.bfloat16).split([4, K, K], 2)
+    # the last one has no token, and lies behind the table
+    for counts, ok in ((None, [True, True, False, False, False]), ([3, 2, 2, 1, 0], [True, True, True, False, True])):
+        start, c = torch.tensor([50, 97, 98, 100, 120], device="cuda"), None if counts is None else torch.tensor(counts, device="cuda")
+        got = kv4_append(cache, k, v, start, c, q=q, table=table)
+        assert lib.ternaspmm_last_status() == 1
+        fine = torch.tensor(ok, device="cuda")
+        for a, b in zip(cache._tensors(), before):
+            assert torch.equal(a[~fine], b[~fine]) and not torch.equal(a[:2], b[:2])
+        assert got[~fine, ..., :n].isnan().all()
+        want, _ = rotate(q[:2], None, table, start[:2, None] + torch.arange(T, device="cuda"))
+        assert torch.equal(got[:2], want)
+        lib.ternaspmm_last_status()
+        for b in range(2):                               # those that fit are there, without a number that is not finite
+            at = slice(int(start[b]), int(start[b]) + (T if counts is None else counts[b]))
+            assert cache.k_scales[b, :, at].isfinite().all() and not torch.equal(cache.v_codes[b, :, at], before[2][b, :, at])
+        out = kv4_attend(got, cache, start, c)
+        assert out[~fine].isnan().all() and out[:2].isfinite().all()
+        for a, b in zip(cache._tensors(), before):
+            a.copy_(b)
+        lib.ternaspmm_last_status()
+    start = torch.tensor([50, 97, 98, 100, 120], device="cuda")
+    kv4_append(cache, k, v, start)                       # without a table every position of the cache is one
+    assert lib.ternaspmm_last_status() == 0 and not torch.equal(cache.k_codes[4], before[0][4])
