@@ -717,7 +717,9 @@ __global__ void __launch_bounds__(256) logprob_grad_kernel(const LogprobGradPara
     const T* row = static_cast<const T*>(p.logits) + (long long)r * p.ld;
     T* out = static_cast<T*>(p.grad) + r * (size_t)p.vocab;
     const long long t = p.targets[r];
-    const float g = p.g_logprob && t >= 0 ? p.g_logprob[r] : 0.f, h = p.g_entropy ? p.g_entropy[r] : 0.f;
+    // (a token outside of the vocabulary has log probability NaN, and so has the gradient that comes through it)
+    const float given = p.g_logprob && t >= 0 ? p.g_logprob[r] : 0.f, g = t >= p.vocab && given != 0.f ? __int_as_float(0x7fffffff) : given;
+    const float h = p.g_entropy ? p.g_entropy[r] : 0.f;
     const float hi = p.lse[2 * r], lo = p.lse[2 * r + 1], ent = p.entropy[r];
     auto one = [&](int j, float x) {
         const float lp = (x - hi) - lo, e = ex2_approx(lp * kLog2e);

@@ -92,3 +92,23 @@ def test_append_beyond_the_table(lib, layout, n):
     start = torch.tensor([50, 97, 98, 100, 120], device="cuda")
     kv4_append(cache, k, v, start)                       # without a table every position of the cache is one
     assert lib.ternaspmm_last_status() == 0 and not torch.equal(cache.k_codes[4], before[0][4])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [300, 20000])
+def test_gradient_of_a_target_outside_of_the_vocabulary(lib, dtype, V):
+    """Its log probability is NaN, and so is the gradient through it; other rows, and the gradient through the entropy alone, are as they are."""
+    x = torch.randn((4, V), generator=gen(V), device="cuda").to(dtype).requires_grad_()
+    t, good = torch.tensor([5, V, -1, 2 ** 40], device="cuda"), torch.tensor([5, 0, -1, 0], device="cuda")
+    w = torch.tensor([1.0, -0.5, 2.0, 0.25], device="cuda")
+    want = torch.autograd.grad((token_logprobs(x, good).logprob * w).sum(), x)[0]
+    assert lib.ternaspmm_last_status() == 0
+    got = torch.autograd.grad((token_logprobs(x, t).logprob * w).sum(), x)[0]
+    assert lib.ternaspmm_last_status() == 1
+    assert got[[1, 3]].isnan().all() and torch.equal(got[[0, 2]], want[[0, 2]])
+    entropy = [torch.autograd.grad((token_logprobs(x, y).entropy * w).sum(), x)[0] for y in (good, t)]
+    assert torch.equal(*entropy) and entropy[0].isfinite().all()
+    r = token_logprobs(x, t)                             # a program that takes the bad rows out
+    got = torch.autograd.grad((torch.where(t < V, r.logprob, 0) * w).sum(), x)[0]
+    assert torch.equal(got, torch.where((t < V)[:, None], want, 0))
+    lib.ternaspmm_last_status()
