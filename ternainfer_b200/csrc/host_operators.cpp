@@ -2,7 +2,7 @@
 // workspaces, the current stream and the autograd nodes in one native call.  Done in Python - a dozen checks, torch.empty, ctypes with
 // some twenty arguments, a Python autograd node - the host side of a call took 27 - 41 us (177 us with its gradient).
 //
-// Wrong arguments raise ValueError, CPU tensors and failed launches RuntimeError.
+// Wrong arguments raise ValueError, CPU tensors and failed launches RuntimeError, tensors with a forward-mode tangent NotImplementedError.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -34,9 +34,12 @@ int type_code(const Tensor& t) {
 
 bool wants_grad(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 
+// (no call has a forward-mode derivative: a tangent that it dropped would count as zero)
 const Tensor& tensor_arg(PyObject* o, const char* name) {
     TORCH_CHECK_TYPE(THPVariable_Check(o), name, " is a tensor, not ", Py_TYPE(o)->tp_name);
-    return THPVariable_Unpack(o);
+    const Tensor& t = THPVariable_Unpack(o);
+    TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), name, " has a tangent: no forward-mode derivative here");
+    return t;
 }
 OptTensor optional_arg(PyObject* o, const char* name) { return o == Py_None ? OptTensor() : OptTensor(tensor_arg(o, name)); }
 

@@ -107,3 +107,21 @@ def test_logprob_statuses(lib):
     grad = dict(x=P, ld=10, type=2, t=P, rows=1, vocab=10, lse=P, h=P, gl=None, gh=P, out=P)
     for status, change in ((1, dict(rows=0)), (1, dict(ld=9)), (2, dict(out=P + 2)), (2, dict(h=None))):
         assert lib.ternaspmm_token_logprobs_grad(*{**grad, **change}.values(), None) == status, change
+
+
+def test_forward_mode_is_refused():
+    """A tensor with a tangent but no gradient of its own: an error, not a result whose tangent counts as zero."""
+    import torch.autograd.forward_ad as forward_ad
+    x, pos = torch.zeros((1, 2, 1, 64), dtype=torch.bfloat16), torch.zeros(2, dtype=torch.int64)
+    table, cache = rotary_table(64, 8, device="cpu"), KV4Cache.empty(1, 1, 64, 64, device="cpu")
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        cos = forward_ad.make_dual(table.cos, torch.ones_like(table.cos))
+        logits = forward_ad.make_dual(torch.zeros((2, 5)), torch.ones((2, 5)))
+        for call in (lambda: rotate(d, None, table, pos), lambda: rotate(x, d, table, pos), lambda: rotate(x, None, RotaryTable(cos, table.sin), pos),
+                     lambda: kv4_append(cache, d, x, pos[:1]), lambda: kv4_append(cache, x, d, pos[:1]), lambda: kv4_append(cache, x, x, pos[:1], q=d, table=table),
+                     lambda: kv4_attend(d, cache, pos[:1]), lambda: token_logprobs(logits, pos)):
+            with pytest.raises(NotImplementedError, match="tangent"):
+                call()
+        with pytest.raises(RuntimeError, match="no CPU path"):            # (as before without one)
+            token_logprobs(forward_ad.unpack_dual(logits).primal, pos)
