@@ -343,7 +343,8 @@ class Transformer(nn.Module):
         return token_logprobs(F.linear(self._final_norm(h), self.tok_embeddings.weight), tokens[:, 1:], top)
 
     def forward(self, tokens: torch.Tensor, cache: List[LayerCache], pos: torch.Tensor, greedy_last: bool = False):
-        """tokens [B, T]; pos [T] (device int64) = positions written in the cache.
+        """tokens [B, T]; pos [T] (device int64) = positions written in the cache.  A 4-bit cache takes consecutive ones inside of the rotary table;
+        others give NaN and status 1 of the library, and leave it as it was.
         Returns fp32 logits [B, T, vocab] (model.py:380-386 of the reference); with ``greedy_last``
         only the greedy token of every sequence's last position, int64 [B] (what the generation
         loop needs: generate.py:274, :283, :305 of the reference)."""
@@ -359,7 +360,12 @@ class Transformer(nn.Module):
         fused = self.args.fused_glue and self.tp == 1
         flash, cos, sin, mask = None, None, None, None
         if self.args.kv_bits == 4:
-            pass             # rotation and visibility follow from the first position
+            # Rotation and visibility follow from the first position.  Whether the others are the ones after it only the device knows: where they are not, the
+            # kernels get one that they refuse (status 1, caches as they were).
+            if pos.shape != (T,):
+                raise ValueError(f"positions [{T}] wanted, not {list(pos.shape)}")
+            if T > 1:
+                pos = torch.where((pos == pos[0] + torch.arange(T, device=pos.device)).all(), pos[:1], -1)
         elif self.flash:   # the attention kernels apply RoPE from the tables and mask by position themselves
             flash = (pos, self._rope_lp, tuple(t.index_select(0, pos) for t in self._rope_lp) if T == 1 else None)
         else:

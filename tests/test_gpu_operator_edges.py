@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from test_gpu_kv4 import check as check_attention, filled, levels
+from test_gpu_long_context import build
 from test_gpu_logprobs import TYPES, check as check_scores, gen
 from ternainfer_b200.kv4 import KV4Cache, kv4_append, kv4_attend
 from ternainfer_b200.rotary import rotary_table, rotate
@@ -112,3 +113,31 @@ def test_gradient_of_a_target_outside_of_the_vocabulary(lib, dtype, V):
     got = torch.autograd.grad((torch.where(t < V, r.logprob, 0) * w).sum(), x)[0]
     assert torch.equal(got, torch.where((t < V)[:, None], want, 0))
     lib.ternaspmm_last_status()
+
+
+@torch.inference_mode()
+@pytest.mark.parametrize("fused", [False, True])
+def test_positions_of_the_models_4_bit_cache(lib, fused):
+    """Tokens at consecutive positions inside of the table, from any first one on; others are refused: NaN, status 1, caches as they were."""
+    m = build(max_len=100, kv_bits=4, fused_glue=fused)
+    tok = torch.randint(0, 1024, (2, 12), generator=gen(5), device="cuda")
+    at = torch.arange(12, device="cuda")
+    cache = m.make_cache(2, "cuda")
+    whole = m(tok, cache, at)
+    again = m.make_cache(2, "cuda")
+    m(tok[:, :5], again, at[:5])
+    m(tok[:, 5:], again, at[5:])
+    assert all(torch.equal(a, b) for x, y in zip(cache[:1], again[:1]) for a, b in zip(x._tensors(), y._tensors())) and lib.ternaspmm_last_status() == 0
+    held = [[t.clone() for t in c._tensors()] for c in cache]
+    for pos in (at.flip(0), at + (at > 6), at * 0 + 3, at + 89, at - 1):
+        out = m(tok, cache, pos)
+        assert lib.ternaspmm_last_status() == 1 and out.isnan().all()
+        assert all(torch.equal(a, b) for c, h in zip(cache, held) for a, b in zip(c._tensors(), h))
+    for pos in (at[:1] + 100, at[:1] + 127, at[:1] - 1):
+        out = m(tok[:, :1], cache, pos)
+        assert lib.ternaspmm_last_status() == 1 and out.isnan().all()
+        assert all(torch.equal(a, b) for c, h in zip(cache, held) for a, b in zip(c._tensors(), h))
+    for pos in (at[:5], at[:, None], torch.arange(13, device="cuda")):
+        with pytest.raises(ValueError):
+            m(tok, cache, pos)
+    assert torch.equal(m(tok, cache, at), whole) and lib.ternaspmm_last_status() == 0
