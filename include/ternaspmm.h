@@ -364,7 +364,8 @@ int ternaspmm_kv4_read(void* k_codes, void* k_scales, void* v_codes, void* v_sca
 /* Attention of the new tokens (already appended, queries already rotated) over the cache: the query of token t, at position p =
  * start + t, sees the keys j <= p below start + count, with window > 0 only those above p - window.  A row that sees none is zero.
  * Calls of several tokens may hold keys and values as fp16: their values beyond 65504 (and NaN scales) make NaN in their group of 32 for the rows
- * that see them, and 2^-11 is the error of each.  scale: of the scores, > 0 and at most 1e6.  out bf16 [batch][tokens][heads][head_dim].  q, out 16-byte aligned, strides of q multiples of 8, heads
+ * that see them, and 2^-11 is the error of each.  scale: of the scores, > 0 and at most 1e6; scores beyond 2e7 in magnitude, where fp32 tells no
+ * differences of 1 apart, may give NaN.  out bf16 [batch][tokens][heads][head_dim].  q, out 16-byte aligned, strides of q multiples of 8, heads
  * a multiple of kv_heads.  workspace: ternaspmm_kv4_attend_workspace() bytes (may be 0; -1: shape not taken), 16-byte
  * aligned, not shared by calls that may overlap on the GPU. */
 int ternaspmm_kv4_attend(const ternaspmm_bf16* q, const long long* q_strides, void* k_codes, void* k_scales, void* v_codes,

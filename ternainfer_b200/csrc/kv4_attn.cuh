@@ -120,6 +120,11 @@ __device__ __forceinline__ void kv4_store(const Kv4AttnParams& p, bool ok, int b
     *reinterpret_cast<uint2*>(p.out + (((size_t)b * p.tokens + row / per_kv) * p.heads + hk * per_kv + row % per_kv) * dim + d) = w;
 }
 
+// What a row's raw scores are multiplied by, kept from 0 and infinity (the product of a tiny or huge scale and query): -inf, of a key that is not
+// seen, and 0 must stay what they are.  Raw scores are below 2^45 (queries 2^15, codes less 8, scales 2^16, 128 of them), so what the lower
+// border changes is far below a rounding of 1; at the upper one a score that is not 0 is beyond what a difference of 1 can be told from.
+__device__ __forceinline__ float kv4_row_factor(float f) { return fminf(fmaxf(f, 0x1p-100f), 0x1p127f); }
+
 template <int D>
 struct Kv4Stage {                          // 32 tokens of a head
     static constexpr int G = D / kKv4Group;
@@ -296,7 +301,7 @@ __global__ void __launch_bounds__(kKv4Warps * 32, NT == 1 ? 4 : 2) kv4_attn_kern
         // 2^(14 - exponent of the largest): that one becomes 2^14 .. 2^15
         const int ex = min(max((int)(__float_as_uint(amax) >> 23), 30), 240) - 127;
         const float up = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
-        const float f = p.scale_log2 * __uint_as_float((uint32_t)(127 + 10 + ex) << 23);   // 2^24 / up
+        const float f = kv4_row_factor(p.scale_log2 * __uint_as_float((uint32_t)(127 + 10 + ex) << 23));   // 2^24 / up
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             row_f[nt][n] = __shfl_sync(0xffffffffu, f, (2 * q + n) * 4);

@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
             }
             const int ex = min(max((int)(__float_as_uint(amax) >> 23), 30), 240) - 127;      // the largest becomes 2^14 .. 2^15
             const float up = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
-            row_f = p.scale_log2 * __uint_as_float((uint32_t)(127 - 14 + ex) << 23);
+            row_f = kv4_row_factor(p.scale_log2 * __uint_as_float((uint32_t)(127 - 14 + ex) << 23));
 #pragma unroll 4
             for (int i = 0; i < D / 8; ++i) {
                 const uint4 w = ldg_128(src + 8 * i);

@@ -86,6 +86,7 @@ def kv4_attend(q: torch.Tensor, cache: KV4Cache, start: torch.Tensor, counts: Op
     """Attention of T new tokens over the cache that holds them already: queries bf16 [B, T, H, D], rotated, H a multiple of Hkv; ``start``
     and ``counts`` as in ``kv4_append``.  The query of token t sees the keys up to position start[b] + t, below start[b] + counts[b],
     and with ``window`` only the last ``window`` of them; a query that sees none gives zeros.  ``scale`` of the scores: 1 / sqrt(D).  bf16
-    [B, T, H, D].  A sequence outside of the cache gives NaN and status 1 of the library.  Calls of several tokens may round the cache's keys and values
-    to fp16: where they are beyond 65504 the rows that see them have NaN."""
+    [B, T, H, D].  A sequence outside of the cache gives NaN and status 1 of the library.  Scores beyond 2 x 10^7 in magnitude, where fp32 tells no
+    differences of 1 apart, may give NaN.  Calls of several tokens may round the cache's keys and values to fp16: where they are beyond 65504 the
+    rows that see them have NaN."""
     return load_host_call().kv4_attend(q, *cache._tensors(), start, counts, window, scale)

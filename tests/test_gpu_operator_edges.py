@@ -141,3 +141,20 @@ def test_positions_of_the_models_4_bit_cache(lib, fused):
         with pytest.raises(ValueError):
             m(tok, cache, pos)
     assert torch.equal(m(tok, cache, at), whole) and lib.ternaspmm_last_status() == 0
+
+
+@pytest.mark.parametrize("T,past", [(1, 300), (3, 40), (160, 2000)])
+def test_attention_at_the_ends_of_the_scales_range(lib, T, past):
+    """Scores that are nothing beside their softmax, and queries of zeros: the mean of what a row sees, keys that it does not see left out."""
+    B, H, K, D = 2, 8, 2, 64
+    cache, k, v = filled(B, K, past + T + 70, D, 5)
+    start = torch.tensor([past, past // 2], device="cuda")
+    q = torch.randn((B, T, H, D), generator=gen(6), device="cuda").to(torch.bfloat16)
+    q[:, :, 1], q[:, :, 2] = 0, 2.0 ** -100
+    for scale in (1e-10, 1e-13, 1e-25, 1e-37):
+        check_attention(q, cache, k, v, start, scale=scale)
+    check_attention(q, cache, k, v, start, window=33, scale=1e-30)
+    cache.k_scales.zero_()                               # the largest scale and queries, and keys of zeros
+    big = (q.double() * 2.0 ** 100).to(torch.bfloat16)
+    check_attention(big, cache, k * 0, v, start, scale=1e6)
+    assert lib.ternaspmm_last_status() == 0
