@@ -376,7 +376,7 @@ long long ternaspmm_kv4_attend_workspace(int batch, int tokens, int heads, int k
 
 /* Per row of logits [rows][vocab] (type as above, `ld` elements between rows): log probability of targets[row] (int64; negative: no
  * token, 0), entropy, log of the sum of exponentials (lse fp32 [rows][2], two parts, for _grad), and the `top` <= 32 most probable tokens with their log probabilities, the lowest id
- * first among equal logits (NaN before all).  _grad: grad [rows][vocab] contiguous, of the logits' type, from the gradients of log probability
+ * first among equal logits (NaN before all).  vocab up to 2^19, rows up to 2^23 where a row is longer than 32 KB.  _grad: grad [rows][vocab] contiguous, of the logits' type, from the gradients of log probability
  * and entropy (either may be null); NaN in a row whose target is `vocab` or above and whose gradient of the log probability is not 0. */
 int ternaspmm_token_logprobs(const void* logits, long long ld, int type, const long long* targets, int rows, int vocab, int top,
                              float* logprob, float* entropy, float* lse, float* top_logprob, long long* top_token, void* workspace,

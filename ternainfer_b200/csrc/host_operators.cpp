@@ -314,7 +314,7 @@ Scores scores_launch(const Tensor& logits, const Tensor& targets, int64_t top) {
     float* stats = as<float>(s.stats);
     if (N) {
         const long long need = ternaspmm_token_logprobs_workspace((int)N, (int)V, type_code(logits), (int)top);
-        TORCH_CHECK_VALUE(need >= 0, "token_logprobs: a vocabulary of ", V, " (up to 2^19)");
+        TORCH_CHECK_VALUE(need >= 0, "token_logprobs: ", N, " rows of ", V, " logits (2^19 at most; 2^23 rows where a row is longer than 32 KB)");
         const Tensor work = at::empty({need}, logits.options().dtype(at::kByte));   // of this call alone
         launched(ternaspmm_token_logprobs(ptr(rows), row_step(rows), type_code(logits), as<long long>(ids), (int)N, (int)V, (int)top, stats, stats + N,
                                           stats + 2 * N, top ? as<float>(s.top_logprob) : nullptr, top ? as<long long>(s.top_token) : nullptr, ptr(work), need,

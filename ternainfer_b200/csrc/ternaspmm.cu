@@ -1470,7 +1470,9 @@ static bool logprob_by_rows(int rows, int vocab, int type, int top) {
     return logprob_parts(vocab, type) == 1 && (rows >= 10 * device_sm_count() || bytes <= 8192 || top > bytes / 1024);
 }
 static bool logprob_shape(int rows, int vocab, int type, int top) {
-    return rows >= 1 && rows <= (1 << 23) && vocab >= 1 && vocab <= kLpMaxVocab && type >= 0 && type <= 2 && top >= 0 && top <= kLpMaxTop && top <= vocab;
+    // (as many as 2^23 rows of several parts are more than the card holds, and than the launch counts in 32 bits)
+    return rows >= 1 && vocab >= 1 && vocab <= kLpMaxVocab && type >= 0 && type <= 2 && top >= 0 && top <= kLpMaxTop && top <= vocab &&
+           (rows <= (1 << 23) || logprob_parts(vocab, type) == 1);
 }
 
 extern "C" long long ternaspmm_token_logprobs_workspace(int rows, int vocab, int type, int top) {
@@ -1483,7 +1485,7 @@ template <typename T>
 static cudaError_t launch_logprobs(const LogprobParams& p, cudaStream_t stream) {
     if (logprob_by_rows(p.rows, p.vocab, std::is_same<T, float>::value ? 2 : 0, p.top)) {
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)((p.rows + kLpWarps - 1) / kLpWarps), 1, 1);
+        cfg.gridDim = dim3((unsigned)((p.rows + (long long)kLpWarps - 1) / kLpWarps), 1, 1);
         cfg.blockDim = dim3(kLpThreads, 1, 1);
         cfg.stream = stream;
         return cudaLaunchKernelEx(&cfg, logprob_rows_kernel<T>, p);

@@ -158,3 +158,15 @@ def test_attention_at_the_ends_of_the_scales_range(lib, T, past):
     big = (q.double() * 2.0 ** 100).to(torch.bfloat16)
     check_attention(big, cache, k * 0, v, start, scale=1e6)
     assert lib.ternaspmm_last_status() == 0
+
+
+def test_more_than_2_23_short_rows(lib):
+    N, V = (1 << 23) + 9, 3
+    x = torch.randn((N, V), generator=gen(1), device="cuda")
+    t = torch.randint(-1, V, (N,), generator=gen(2), device="cuda")
+    check_scores(x, t, 2)
+    x.requires_grad_()
+    got, = torch.autograd.grad(token_logprobs(x, t).logprob.sum(), x)
+    tail = x.detach()[-5:].clone().requires_grad_()
+    assert torch.equal(got[-5:], torch.autograd.grad(token_logprobs(tail, t[-5:]).logprob.sum(), tail)[0])
+    assert lib.ternaspmm_last_status() == 0

@@ -125,3 +125,9 @@ def test_forward_mode_is_refused():
                 call()
         with pytest.raises(RuntimeError, match="no CPU path"):            # (as before without one)
             token_logprobs(forward_ad.unpack_dual(logits).primal, pos)
+
+
+def test_logprob_rows(lib):
+    many = (1 << 23) + 1
+    assert lib.ternaspmm_token_logprobs_workspace(many, 1 << 14, 0, 0) == 16 == lib.ternaspmm_token_logprobs_workspace((1 << 31) - 1, 1 << 13, 2, 0)
+    assert lib.ternaspmm_token_logprobs_workspace(many, (1 << 14) + 1, 0, 0) == -1 == lib.ternaspmm_token_logprobs_workspace(1, (1 << 31) - 1, 0, 0)
