@@ -334,14 +334,15 @@ int ternaspmm_attn_prefill(ternaspmm_bf16* qkv, ternaspmm_bf16* k_cache, ternasp
  * head, or (i, i + rotary_dim / 2) with half_layout; (a, b) -> (a c - b s, a s + b c), the rest is copied.  inverse: -s (the
  * gradient).  type: 0 bf16, 1 fp16, 2 fp32.  cos_tab, sin_tab fp32 [table_len][rotary_dim / 2]; pos int64, `pos_batch_stride` and
  * `pos_token_stride` elements apart (0: shared).  q_out, k_out contiguous.  Any strides in the half layout; even ones, and pointers to whole pairs, in
- * the other.  head_dim and rotary_dim even. */
+ * the other.  head_dim and rotary_dim even.  Status 1 also for more than 2^31 pieces (16 bytes of one to four heads, where
+ * pointers and strides are not multiples of 16 bytes one or two values). */
 int ternaspmm_rotate(const void* q, const long long* q_strides, int q_heads, void* q_out, const void* k, const long long* k_strides,
                      int k_heads, void* k_out, int type, const float* cos_tab, const float* sin_tab, int table_len, int rotary_dim,
                      int half_layout, int inverse, const long long* pos, long long pos_batch_stride, long long pos_token_stride,
                      int batch, int tokens, int head_dim, ternaspmm_stream_t stream);
 
 /* The cache: codes uint8 [batch][kv_heads][max_len][head_dim / 2] and scales fp16 [batch][kv_heads][max_len][head_dim / 32] of keys
- * and of values, 16-byte aligned; head_dim 64 or 128, max_len a multiple of 64.  A group of 32 values shares scale = fp16(m / -8), m its
+ * and of values, 16-byte aligned; head_dim 64 or 128, max_len a multiple of 64, batch up to 65535.  A group of 32 values shares scale = fp16(m / -8), m its
  * value of largest magnitude (the positive one of two); code = clamp(rint(x / scale) + 8, 0, 15) stands for scale * (code - 8).
  * Codes are packed two a byte, the even one low; a key row then holds 4-byte word t of every group, t = 0 .. 3, a value row 2-byte
  * halfword g of every group, g = 0 .. 7.

@@ -52,7 +52,10 @@ long long int_arg(PyObject* o, const char* name) {
 
 void on_gpu(const Tensor& t, const char* what) { TORCH_CHECK(t.is_cuda(), what, " needs CUDA tensors: the B200 library has no CPU path"); }
 
-void launched(int status, const char* what) { TORCH_CHECK(status == 0, what, ": status ", status); }
+void launched(int status, const char* what) {
+    TORCH_CHECK_VALUE(status != 1 && status != 2, what, status == 1 ? ": more than a launch takes" : ": pointers off their boundaries");
+    TORCH_CHECK(status == 0, what, ": status ", status);
+}
 
 void* ptr(const Tensor& t) { return t.data_ptr(); }
 void* ptr(const OptTensor& t) { return t ? t->data_ptr() : nullptr; }

@@ -1178,7 +1178,8 @@ static cudaError_t launch_rotate_heads(RotateParams p, long long tokens_all, cud
     const int turned = HALF ? p.rotary / 2 / V : p.rotary / V, units = turned + (p.dim - p.rotary) / V;
     const int head_groups = (p.q.heads + p.k.heads + HEADS - 1) / HEADS;
     const long long items = tokens_all * head_groups * units;
-    if (items >= 0x7fffffffll - 256) return cudaErrorInvalidValue;
+    if (items >= 0x7fffffffll - 256) return cudaErrorNotSupported;
+    if (!p.status) return cudaErrorNoDevice;
     p.units = FastDiv(units), p.head_groups = FastDiv(head_groups);
     p.tables_16 = (p.rotary / 2) % 4 == 0 && ((reinterpret_cast<uintptr_t>(p.cos_tab) | reinterpret_cast<uintptr_t>(p.sin_tab)) & 15) == 0;
     cudaLaunchConfig_t cfg = {};
@@ -1222,7 +1223,6 @@ extern "C" int ternaspmm_rotate(const void* q, const long long* q_strides, int q
     const uintptr_t bits = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(k_out);
     if (!q || !q_strides || !q_out || (k_heads && (!k || !k_strides || !k_out)) || !cos_tab || !sin_tab || !pos || bits % size)
         return t_host_status = ST_BAD_POINTER;
-    if (!status) return t_host_status = ST_LAUNCH;
     RotateParams p = {};
     p.q = {q, q_out, q_strides[0], q_strides[1], q_strides[2], q_heads};
     if (k_heads) p.k = {k, k_out, k_strides[0], k_strides[1], k_strides[2], k_heads};
@@ -1233,6 +1233,7 @@ extern "C" int ternaspmm_rotate(const void* q, const long long* q_strides, int q
     const cudaError_t e = type == 0 ? launch_rotate_type<__nv_bfloat16>(p, all, half_layout != 0, stream)
                           : type == 1 ? launch_rotate_type<__half>(p, all, half_layout != 0, stream) : launch_rotate_type<float>(p, all, half_layout != 0, stream);
     if (e == cudaErrorMisalignedAddress) return t_host_status = ST_BAD_POINTER;
+    if (e == cudaErrorNotSupported) return t_host_status = ST_BAD_SHAPE;   // more than a launch takes
     return launch_result(e);
 }
 

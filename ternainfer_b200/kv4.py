@@ -16,6 +16,7 @@ from .rotary import RotaryTable
 
 GROUP = 32                # values that share a scale
 TILE = 64                 # the capacity is a multiple of this
+MAX_BATCH = 65535         # sequences of a cache
 
 
 @dataclass(frozen=True)
@@ -33,8 +34,8 @@ class KV4Cache:
                             (self.v_scales, torch.float16, half // 16)):
             if t.dtype != dtype or tuple(t.shape) != (B, H, L, n) or not t.is_contiguous() or t.device != self.k_codes.device or t.data_ptr() % 16:
                 raise ValueError("codes are contiguous uint8 [B, Hkv, L, D / 2], scales fp16 [B, Hkv, L, D / 32], all on one device")
-        if half not in (32, 64) or L % TILE or L == 0 or B == 0 or H == 0:
-            raise ValueError(f"heads have 64 or 128 values and the capacity is a multiple of {TILE}: not {2 * half}, {L}")
+        if half not in (32, 64) or L % TILE or L == 0 or H == 0 or not 0 < B <= MAX_BATCH:
+            raise ValueError(f"heads have 64 or 128 values, the capacity is a multiple of {TILE} and there are 1 to {MAX_BATCH} sequences: not {2 * half}, {L}, {B}")
 
     @classmethod
     def empty(cls, batch: int, kv_heads: int, max_len: int, head_dim: int, device="cuda") -> "KV4Cache":

@@ -127,6 +127,15 @@ def test_forward_mode_is_refused():
             token_logprobs(forward_ad.unpack_dual(logits).primal, pos)
 
 
+def test_sizes_that_no_launch_takes(lib):
+    rotate_args = dict(q=P, qs=strides(6, 6, 6), qh=2, qo=P, k=None, ks=None, kh=0, ko=None, type=0, cos=P, sin=P, len=4, rot=2, half=1, inv=0, pos=P, sb=0, st=1,
+                       batch=1, tokens=1 << 30, dim=6)
+    assert lib.ternaspmm_rotate(*rotate_args.values(), None) == 1 and lib.ternaspmm_last_status() == 1
+    with pytest.raises(ValueError, match="65536"):
+        KV4Cache.empty(65536, 1, 64, 64, device="meta")
+    assert KV4Cache.empty(65535, 1, 64, 64, device="meta").batch == 65535
+
+
 def test_logprob_rows(lib):
     many = (1 << 23) + 1
     assert lib.ternaspmm_token_logprobs_workspace(many, 1 << 14, 0, 0) == 16 == lib.ternaspmm_token_logprobs_workspace((1 << 31) - 1, 1 << 13, 2, 0)
