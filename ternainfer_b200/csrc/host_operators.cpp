@@ -67,8 +67,12 @@ struct Strides {
     explicit Strides(const Tensor& t) : v{t.stride(0), t.stride(1), t.stride(2)} {}
 };
 
+// What a kernel reads is memory: a tensor that torch marks as the negative of its memory (imaginary parts of conjugates, as gradients come) is written out.
+Tensor plain(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 // t with contiguous heads whose rows start on multiples of `bytes`
-Tensor rows_on(const Tensor& t, int bytes) {
+Tensor rows_on(const Tensor& given, int bytes) {
+    const Tensor t = plain(given);
     const int64_t step = bytes / t.element_size();
     const bool ok = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % bytes == 0 && t.stride(0) % step == 0 &&
                     t.stride(1) % step == 0 && t.stride(2) % step == 0;
@@ -293,7 +297,8 @@ PyObject* py_kv4_attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
 // ---------------------------------------------------------------------------------------------------- log probabilities
 
 // Logits as rows [N, V] of contiguous elements, any distance apart.
-Tensor logit_rows(const Tensor& x) {
+Tensor logit_rows(const Tensor& given) {
+    const Tensor x = plain(given);
     const int64_t V = x.size(-1);
     Tensor r = x.dim() == 2 ? x : x.reshape({x.numel() / V, V});
     return (V == 1 || r.stride(1) == 1) && (r.size(0) <= 1 || r.stride(0) >= V) ? r : r.contiguous();
@@ -355,7 +360,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
         const Tensor grad = at::empty({N, V}, rows.options());
         OptTensor g[2];
         for (int i = 0; i < 2; ++i)
-            if (grads[i].defined()) g[i] = grads[i].contiguous();
+            if (grads[i].defined()) g[i] = plain(grads[i]).contiguous();
         float* s = as<float>(stats);
         if (N)
             launched(ternaspmm_token_logprobs_grad(ptr(rows), row_step(rows), type_code(rows), as<long long>(ids), (int)N, (int)V, s + 2 * N, s + N, as<float>(g[0]),

@@ -170,3 +170,12 @@ def test_more_than_2_23_short_rows(lib):
     tail = x.detach()[-5:].clone().requires_grad_()
     assert torch.equal(got[-5:], torch.autograd.grad(token_logprobs(tail, t[-5:]).logprob.sum(), tail)[0])
     assert lib.ternaspmm_last_status() == 0
+
+
+def test_gradients_that_arrive_lazily_negated(lib):
+    """Of one row: where torch hands the gradient of an imaginary part on as a view whose sign is a mark."""
+    x = torch.randn((1, 200), generator=gen(1), device="cuda", requires_grad=True)
+    r = token_logprobs(x, torch.tensor([3], device="cuda"))
+    want, = torch.autograd.grad(r.entropy.sum(), x, retain_graph=True)
+    z = (torch.complex(r.logprob, r.entropy).conj() * 1j).real                # the entropy itself
+    assert torch.equal(z, r.entropy) and torch.equal(torch.autograd.grad(z.sum(), x)[0], want)
