@@ -41,6 +41,13 @@ const Tensor& tensor_arg(PyObject* o, const char* name) {
     TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), name, " has a tangent: no forward-mode derivative here");
     return t;
 }
+// One that the calls treat as given: tables and caches have no gradient, and one that is asked for is not dropped silently.
+const Tensor& constant_arg(PyObject* o, const char* name) {
+    const Tensor& t = tensor_arg(o, name);
+    TORCH_CHECK(!wants_grad(t), name, " requires a gradient: the calls have none for it");
+    return t;
+}
+OptTensor optional_constant(PyObject* o, const char* name) { return o == Py_None ? OptTensor() : OptTensor(constant_arg(o, name)); }
 OptTensor optional_arg(PyObject* o, const char* name) { return o == Py_None ? OptTensor() : OptTensor(tensor_arg(o, name)); }
 
 long long int_arg(PyObject* o, const char* name) {
@@ -151,7 +158,7 @@ variable_list rotate_any(const Tensor& q, const OptTensor& k, const RotaryArgs& 
 PyObject* py_rotate(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     TORCH_CHECK_TYPE(n == 6, "rotate(q, k, cos, sin, half, positions)");
-    const Tensor &q = tensor_arg(args[0], "q"), &cos = tensor_arg(args[2], "cos"), &sin = tensor_arg(args[3], "sin"), &pos = tensor_arg(args[5], "positions");
+    const Tensor &q = tensor_arg(args[0], "q"), &cos = constant_arg(args[2], "cos"), &sin = constant_arg(args[3], "sin"), &pos = tensor_arg(args[5], "positions");
     const OptTensor k = optional_arg(args[1], "k");
     on_gpu(q, "rotate");
     TORCH_CHECK_VALUE(q.dim() == 4 && type_code(q) >= 0 && q.size(3) % 2 == 0, "q is bf16, fp16 or fp32 [B, T, H, D] with an even D, not ", q.scalar_type(), " ",
@@ -176,8 +183,8 @@ struct Cache {
     const Tensor &k_codes, &k_scales, &v_codes, &v_scales;
     int64_t batch, kv_heads, max_len, head_dim;
     explicit Cache(PyObject* const* args)
-        : k_codes(tensor_arg(args[0], "k_codes")), k_scales(tensor_arg(args[1], "k_scales")), v_codes(tensor_arg(args[2], "v_codes")),
-          v_scales(tensor_arg(args[3], "v_scales")), batch(k_codes.size(0)), kv_heads(k_codes.size(1)), max_len(k_codes.size(2)),
+        : k_codes(tensor_arg(args[0], "k_codes")), k_scales(constant_arg(args[1], "k_scales")), v_codes(tensor_arg(args[2], "v_codes")),
+          v_scales(constant_arg(args[3], "v_scales")), batch(k_codes.size(0)), kv_heads(k_codes.size(1)), max_len(k_codes.size(2)),
           head_dim(2 * k_codes.size(3)) {
         TORCH_CHECK_VALUE(std::max({batch, kv_heads, max_len}) <= INT_MAX, "cache of ", k_codes.sizes());
     }
@@ -207,7 +214,7 @@ PyObject* py_kv4_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
     TORCH_CHECK_TYPE(n == 12, "kv4_append(k_codes, k_scales, v_codes, v_scales, k, v, start, counts, q, cos, sin, half)");
     const Cache c(args);
     const Tensor &k0 = tensor_arg(args[4], "k"), &v0 = tensor_arg(args[5], "v"), &start = tensor_arg(args[6], "start");
-    const OptTensor counts = optional_arg(args[7], "counts"), q0 = optional_arg(args[8], "q"), cos = optional_arg(args[9], "cos"), sin = optional_arg(args[10], "sin");
+    const OptTensor counts = optional_arg(args[7], "counts"), q0 = optional_arg(args[8], "q"), cos = optional_constant(args[9], "cos"), sin = optional_constant(args[10], "sin");
     check_rows(c, "k", k0, c.kv_heads);
     check_rows(c, "v", v0, c.kv_heads);
     TORCH_CHECK_VALUE(v0.size(1) == k0.size(1), "k and v have one shape, not ", k0.sizes(), " and ", v0.sizes());

@@ -140,3 +140,19 @@ def test_logprob_rows(lib):
     many = (1 << 23) + 1
     assert lib.ternaspmm_token_logprobs_workspace(many, 1 << 14, 0, 0) == 16 == lib.ternaspmm_token_logprobs_workspace((1 << 31) - 1, 1 << 13, 2, 0)
     assert lib.ternaspmm_token_logprobs_workspace(many, (1 << 14) + 1, 0, 0) == -1 == lib.ternaspmm_token_logprobs_workspace(1, (1 << 31) - 1, 0, 0)
+
+
+def test_gradients_of_tables_and_caches_are_refused():
+    x, pos = torch.zeros((1, 2, 1, 64), dtype=torch.bfloat16), torch.zeros(2, dtype=torch.int64)
+    plain, c = rotary_table(64, 8, device="cpu"), KV4Cache.empty(1, 1, 64, 64, device="cpu")
+    leaf = lambda t: t.clone().requires_grad_()
+    for table in (RotaryTable(leaf(plain.cos), plain.sin), RotaryTable(plain.cos, leaf(plain.sin))):
+        for call in (lambda: rotate(x, None, table, pos), lambda: kv4_append(c, x, x, pos[:1], table=table)):
+            with pytest.raises(RuntimeError, match="requires a gradient"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):
+                call()
+    for cache in (KV4Cache(c.k_codes, leaf(c.k_scales), c.v_codes, c.v_scales), KV4Cache(c.k_codes, c.k_scales, c.v_codes, leaf(c.v_scales))):
+        for call in (lambda: kv4_append(cache, x, x, pos[:1]), lambda: kv4_read(cache, pos[:1], 2), lambda: kv4_attend(x, cache, pos[:1])):
+            with pytest.raises(RuntimeError, match="requires a gradient"):
+                call()
