@@ -112,11 +112,15 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
 }
 template <bool V> struct Kv4Const { static constexpr bool value = V; };
 
-// Four dimensions of a query row: val / sum as bf16; zero for a row that saw no key, NaN for a sequence outside of the cache.
-__device__ __forceinline__ void kv4_store(const Kv4AttnParams& p, bool ok, int b, int hk, int per_kv, int row, int d, float4 val, float sum) {
+// Whether a query at `pos` sees a key at all.
+__device__ __forceinline__ bool kv4_sees(const Kv4Range& r, int pos, int window) { return min(pos, r.limit - 1) >= (window > 0 ? max(pos - window + 1, 0) : 0); }
+
+// Four dimensions of a query row at position `pos`: val / sum as bf16; zero for a row that sees no key, NaN for one that sees keys but has a sum of 0 (every
+// score is -inf: infinite keys or queries), and for a sequence outside of the cache.
+__device__ __forceinline__ void kv4_store(const Kv4AttnParams& p, const Kv4Range& r, int pos, int b, int hk, int per_kv, int row, int d, float4 val, float sum) {
     const int dim = 2 * (int)p.row_bytes;
-    const float inv = sum == 0.f ? 0.f : 1.f / sum, nan = __int_as_float(0x7fffffff);
-    const uint2 w = ok ? make_uint2(bf16_pack(val.x * inv, val.y * inv), bf16_pack(val.z * inv, val.w * inv)) : make_uint2(bf16_pack(nan, nan), bf16_pack(nan, nan));
+    const float nan = __int_as_float(0x7fffffff), inv = sum == 0.f ? (kv4_sees(r, pos, p.window) ? nan : 0.f) : 1.f / sum;
+    const uint2 w = r.ok ? make_uint2(bf16_pack(val.x * inv, val.y * inv), bf16_pack(val.z * inv, val.w * inv)) : make_uint2(bf16_pack(nan, nan), bf16_pack(nan, nan));
     *reinterpret_cast<uint2*>(p.out + (((size_t)b * p.tokens + row / per_kv) * p.heads + hk * per_kv + row % per_kv) * dim + d) = w;
 }
 
@@ -557,7 +561,7 @@ __global__ void __launch_bounds__(kKv4Warps * 32, NT == 1 ? 4 : 2) kv4_attn_kern
             if (d == 0) cta_ml[r] = make_float2(top, sum);
         } else if (r0 + r < rows_all) {
             if (whole) {
-                kv4_store(p, rg.ok, b, hk, per_kv, r0 + r, d, val, sum);
+                kv4_store(p, rg, rg.first_pos - t_first + (r0 + r) / per_kv, b, hk, per_kv, r0 + r, d, val, sum);
             } else {
                 const size_t at = (size_t)(2 * blockIdx.x + (first_part ? 0 : 1)) * ROWS + r;
                 *reinterpret_cast<float4*>(p.part_o + at * D + d) = val;
@@ -592,7 +596,7 @@ __global__ void __launch_bounds__(kKv4Warps * 32, NT == 1 ? 4 : 2) kv4_attn_kern
                     sum += f * st[c].y;
                     if (f != 0.f) val.x += f * y[c].x, val.y += f * y[c].y, val.z += f * y[c].z, val.w += f * y[c].w;
                 }
-            kv4_store(p, rg.ok, b, hk, per_kv, r0 + r, d, val, sum);
+            kv4_store(p, rg, rg.first_pos - t_first + (r0 + r) / per_kv, b, hk, per_kv, r0 + r, d, val, sum);
         }
         cluster_arrive();                                          // nobody leaves while its results are read
         cluster_wait();
@@ -673,7 +677,7 @@ __global__ void __launch_bounds__(kKv4JoinWarps * 32) kv4_attn_join_kernel(const
     }
     const Kv4Range rg = kv4_range(p.start, p.counts, p.start_stride, b, p.tokens, p.window, p.c.max_len, 0, p.tokens - 1);
     if (!rg.ok && lane == 0) *p.status = 1;
-    kv4_store(p, rg.ok, b, hk, per_kv, r, lane * 4, val, sum);
+    kv4_store(p, rg, rg.first_pos + r / per_kv, b, hk, per_kv, r, lane * 4, val, sum);
 }
 
 }  // namespace tsp

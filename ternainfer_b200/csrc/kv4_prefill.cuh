@@ -378,6 +378,7 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
         const float nan = __int_as_float(0x7fffffff);
         const bool whole = p.cluster == 1;
         const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
+        const bool none = whole && l == 0.f && kv4_sees(rg, pos, p.window);   // keys, but no score above -inf (as in kv4_store)
         const size_t at = ((size_t)b * gridDim.x + blockIdx.x) * kKvpRows + tid;
         __nv_bfloat16* dst = p.out + (((size_t)b * p.tokens + t) * p.heads + h) * D;
         if (!whole) p.part_ml[at] = make_float2(-nb, ok ? l : nan);
@@ -388,8 +389,8 @@ __global__ void __launch_bounds__(kKvpThreads, 2) kv4_prefill_kernel(const Kv4At
                 tmem_ld32(t_o + mine + c, o);
                 tmem_ld32_wait(o);
             }
-            bool lost = !ok || !rg.ok || seen_to >= bad[c / 32];
-            if (p.window && ok && rg.ok && lost) {                 // (`bad` is the first such key: is there one that this row sees?)
+            bool lost = !ok || !rg.ok || none || seen_to >= bad[c / 32];
+            if (p.window && ok && rg.ok && !none && lost) {                 // (`bad` is the first such key: is there one that this row sees?)
                 lost = false;
                 const __half* vs = p.c.v_scales + (row0 - base) * G + c / 32;
                 for (int key = max(seen_from, base); key <= min(seen_to, base + tiles * kKvpKeys - 1); ++key)
@@ -449,8 +450,8 @@ __global__ void __launch_bounds__(kKvpJoinWarps * 32) kv4_prefill_join_kernel(co
             val.x = val.x * f + y[j].x * g, val.y = val.y * f + y[j].y * g, val.z = val.z * f + y[j].z * g, val.w = val.w * f + y[j].w * g;
         }
     }
-    const bool ok = kv4_range(p.start, p.counts, p.start_stride, b, p.tokens, p.window, p.c.max_len, 0, 0).ok;
-    if (lane < D / 4) kv4_store(p, ok, b, hk, per_kv, row, lane * 4, val, sum);
+    const Kv4Range rg = kv4_range(p.start, p.counts, p.start_stride, b, p.tokens, p.window, p.c.max_len, 0, 0);
+    if (lane < D / 4) kv4_store(p, rg, rg.first_pos + row / per_kv, b, hk, per_kv, row, lane * 4, val, sum);
 }
 
 }  // namespace tsp

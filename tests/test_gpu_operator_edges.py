@@ -179,3 +179,18 @@ def test_gradients_that_arrive_lazily_negated(lib):
     want, = torch.autograd.grad(r.entropy.sum(), x, retain_graph=True)
     z = (torch.complex(r.logprob, r.entropy).conj() * 1j).real                # the entropy itself
     assert torch.equal(z, r.entropy) and torch.equal(torch.autograd.grad(z.sum(), x)[0], want)
+
+
+@pytest.mark.parametrize("window", [0, 70])
+@pytest.mark.parametrize("T,past", [(200, 0), (160, 2000)])
+def test_rows_whose_every_score_is_minus_infinity(lib, T, past, window):
+    """Keys beyond fp16 among many tokens make NaN of the rows that see them, also where all scores are -inf; rows that see no key stay zero."""
+    B, H, K, D = 2, 16, 2, 64
+    cache = KV4Cache.empty(B, K, past + T, D)
+    k = torch.full((B, past + T, K, D), 1e5, device="cuda", dtype=torch.bfloat16)
+    kv4_append(cache, k, torch.ones_like(k), torch.zeros(B, dtype=torch.int64, device="cuda"))
+    q = torch.full((B, T, H, D), -1.0, device="cuda", dtype=torch.bfloat16)
+    start, counts = torch.tensor([past, 0], device="cuda"), torch.tensor([T, 0], device="cuda")
+    out = kv4_attend(q, cache, start, counts, window=window)
+    assert out[0].isnan().all() and not out[1].any()
+    assert lib.ternaspmm_last_status() == 0
