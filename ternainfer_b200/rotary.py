@@ -52,6 +52,8 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: Optiona
                   mixed by their number of turns between."""
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rotary_dim is even and at least 2, not {rotary_dim}")
+    if not theta > 0:
+        raise ValueError(f"theta is above 0, not {theta}")
     pair = torch.arange(rotary_dim // 2, dtype=torch.float64, device=device)
     inv = theta ** (-2 * pair / rotary_dim)
     if scaling is None:
@@ -71,8 +73,12 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: Optiona
     if "original_len" not in scaling:
         raise ValueError(f"{kind} scaling needs original_len")
     length = float(scaling["original_len"])
+    if not length > 0:
+        raise ValueError(f"original_len is above 0, not {length}")
     if kind == "yarn":
         fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
+        if not fast >= slow > 0 or theta == 1:
+            raise ValueError(f"yarn scaling needs beta_fast >= beta_slow > 0 and a theta other than 1, not {fast}, {slow}, {theta}")
 
         def pair_with(turns):                # index of the pair that turns so often over the original length
             return rotary_dim * math.log(length / (2 * math.pi * turns)) / (2 * math.log(theta))

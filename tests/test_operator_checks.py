@@ -156,3 +156,17 @@ def test_gradients_of_tables_and_caches_are_refused():
         for call in (lambda: kv4_append(cache, x, x, pos[:1]), lambda: kv4_read(cache, pos[:1], 2), lambda: kv4_attend(x, cache, pos[:1])):
             with pytest.raises(RuntimeError, match="requires a gradient"):
                 call()
+
+
+def test_frequencies_that_do_not_exist():
+    """Wrong numbers are ValueErrors: no table of NaN, and no division by zero on the way."""
+    for theta in (-10000.0, 0.0, math.nan):
+        with pytest.raises(ValueError, match="theta"):
+            rotary_frequencies(32, theta)
+    yarn = dict(type="yarn", factor=4, original_len=4096)
+    for theta, scaling in ((1.0, yarn), (10000.0, dict(yarn, beta_fast=0)), (10000.0, dict(yarn, beta_slow=0)), (10000.0, dict(yarn, beta_slow=-1)),
+                           (10000.0, dict(yarn, beta_fast=1, beta_slow=32)), (10000.0, dict(yarn, original_len=0)),
+                           (10000.0, dict(type="wavelength", factor=4, original_len=-4096))):
+        with pytest.raises(ValueError, match="yarn|original_len"):
+            rotary_frequencies(32, theta, scaling)
+    assert torch.equal(rotary_frequencies(32, 1.0)[0], torch.ones(16, dtype=torch.float64))
