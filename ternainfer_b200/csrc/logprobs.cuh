@@ -144,10 +144,11 @@ struct LpPart {
     __device__ __forceinline__ int vec(int j, int tid) const { return first + (tid >> 5) * (32 * kLpVecs) + j * 32 + (tid & 31); }
     __device__ __forceinline__ int index(int j, int tid) const { return head + vec(j, tid) * LpVec<T>::N; }   // of a vector's first element
     __device__ __forceinline__ bool has(int j, int tid) const { return vec(j, tid) < vecs; }
-    __device__ __forceinline__ int edge(int tid) const {          // index of this thread's element of the edges, or -1
-        if (part == 0 && tid < head) return tid;
+    __device__ __forceinline__ int edge(int tid) const { return edge(tid, part == 0, part == parts - 1); }
+    __device__ __forceinline__ int edge(int tid, bool front, bool back) const {   // index of this thread's element of the edges, or -1
+        if (front && tid < head) return tid;
         const int rest = head + vecs * LpVec<T>::N + tid - 8;
-        return part == parts - 1 && tid >= 8 && rest < vocab && tid < 16 ? rest : -1;
+        return back && tid >= 8 && rest < vocab && tid < 16 ? rest : -1;
     }
 };
 
@@ -498,7 +499,6 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) logprob_rows_kernel(
     if (r >= (unsigned)p.rows) return;                             // (no barrier of the CTA below)
     unsigned long long* cand = lists[warp];
     LpPart<T> at(p, r, 0);
-    at.parts = max(1, (at.vecs + 32 * kLpVecs - 1) / (32 * kLpVecs));   // pieces of 4 KB: the row's last elements go with the last one, as ids ascend
     const long long target = p.targets[r];
     const float xt = target >= 0 && target < p.vocab ? Elem<T>::get(at.row[target]) : 0.f;
     if (lane == 0) counts[warp] = 0;
@@ -506,8 +506,9 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) logprob_rows_kernel(
     uint32_t bound = 0;
     bool full = false;
 #pragma unroll 1
-    for (int k = 0; k < at.parts; ++k, ++at.part, at.first += 32 * kLpVecs) {
-        const int edge = at.edge(lane), n = min(kLpVecs, (at.vecs - at.first + 31) / 32);
+    for (int k = 0; k == 0 || at.first < at.vecs; ++k, at.first += 32 * kLpVecs) {
+        // (of the edges the row's last elements go with its last 4 KB, as ids ascend)
+        const int edge = at.edge(lane, k == 0, at.first + 32 * kLpVecs >= at.vecs), n = min(kLpVecs, (at.vecs - at.first + 31) / 32);
         auto again = [&](int j) { return at.has(j, lane) ? Vec16{ldg_128(at.row + at.index(j, lane))} : Vec16{make_uint4(Vec16::none, Vec16::none, Vec16::none, Vec16::none)}; };
         Vec16 x16[kLpVecs];
 #pragma unroll
