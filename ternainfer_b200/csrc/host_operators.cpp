@@ -69,9 +69,11 @@ void* ptr(const OptTensor& t) { return t ? t->data_ptr() : nullptr; }
 template <typename T> T* as(const Tensor& t) { return static_cast<T*>(t.data_ptr()); }
 template <typename T> T* as(const OptTensor& t) { return t ? static_cast<T*>(t->data_ptr()) : nullptr; }
 
+// (a dimension of one element has no stride: what torch keeps there can be any number)
+int64_t stride_of(const Tensor& t, int i) { return t.size(i) > 1 ? t.stride(i) : 0; }
 struct Strides {
     long long v[3];
-    explicit Strides(const Tensor& t) : v{t.stride(0), t.stride(1), t.stride(2)} {}
+    explicit Strides(const Tensor& t) : v{stride_of(t, 0), stride_of(t, 1), stride_of(t, 2)} {}
 };
 
 // What a kernel reads is memory: a tensor that torch marks as the negative of its memory (imaginary parts of conjugates, as gradients come) is written out.
@@ -81,11 +83,11 @@ Tensor plain(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
 Tensor rows_on(const Tensor& given, int bytes) {
     const Tensor t = plain(given);
     const int64_t step = bytes / t.element_size();
-    const bool ok = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % bytes == 0 && t.stride(0) % step == 0 &&
-                    t.stride(1) % step == 0 && t.stride(2) % step == 0;
+    const bool ok = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % bytes == 0 && stride_of(t, 0) % step == 0 &&
+                    stride_of(t, 1) % step == 0 && stride_of(t, 2) % step == 0;
     if (ok) return t;
     const Tensor r = t.contiguous();
-    return r.data_ptr() == t.data_ptr() ? t.clone() : r;           // (contiguous, but off the boundary)
+    return r.data_ptr() == t.data_ptr() ? t.clone(at::MemoryFormat::Contiguous) : r;   // (contiguous, but off the boundary)
 }
 
 PyObject* wrap(const Tensor& t) { return THPVariable_Wrap(t); }

@@ -194,3 +194,26 @@ def test_rows_whose_every_score_is_minus_infinity(lib, T, past, window):
     out = kv4_attend(q, cache, start, counts, window=window)
     assert out[0].isnan().all() and not out[1].any()
     assert lib.ternaspmm_last_status() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_strides_of_single_elements_do_not_matter(lib, dtype):
+    """One sequence, token or head of a tensor of odd row lengths: what torch keeps as its stride there is no distance between anything."""
+    table = rotary_table(64, 20)
+    base = torch.randn(4000, generator=gen(1), device="cuda").to(dtype)
+    pos = torch.tensor([7], device="cuda")
+    for shape, strides in (((1, 1, 5, 64), (999, 77, 66, 1)), ((1, 1, 1, 64), (3, 5, 7, 1)), ((3, 1, 1, 64), (200, 1, 13, 1)), ((1, 1, 4, 64), (1, 1, 64, 1))):
+        for offset in (0, 1, 2, 6, 8):
+            x = base.as_strided(shape, strides, offset)
+            for layout in ("interleaved", "half"):
+                y = rotary_table(64, 20, layout=layout)
+                assert torch.equal(rotate(x, x, y, pos)[1], rotate(x.clone(memory_format=torch.contiguous_format), None, y, pos)[0])
+            if dtype != torch.bfloat16:
+                continue
+            B, _, K, D = shape
+            start = torch.full((B,), 7, device="cuda")
+            a, b = (KV4Cache.empty(B, K, 64, D) for _ in range(2))
+            c = x.clone(memory_format=torch.contiguous_format)
+            assert torch.equal(kv4_append(a, x, x, start, q=x, table=table), kv4_append(b, c, c, start, q=c, table=table))
+            assert all(torch.equal(s, t) for s, t in zip(a._tensors(), b._tensors())) and torch.equal(kv4_attend(x, a, start), kv4_attend(c, b, start))
+    assert lib.ternaspmm_last_status() == 0
