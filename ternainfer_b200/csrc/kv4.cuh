@@ -72,7 +72,8 @@ constexpr int kKv4Heads = 4;               // rows of a token that a thread of t
 // A thread takes 8 consecutive values in HEADS heads of a token - queries (rotated into q_out), keys (rotated, quantised), values
 // (quantised) -, all of them on their way before the first is used; four lanes share a group's scale.  Three prompts of 1,226 tokens, 20 + 2 x 5 heads
 // of 128, rotation included, and the reading back of what was written: 26.5 us for 60 MB, of which 9.3 are the bytes; what bounds it is the
-// instructions of a value (pair, maximum, quotient, packing, some 12), at half of the issue slots.  A step of 8 tokens 5.7 us, two chains of latencies.
+// instructions of a value (pair, maximum, quotient, packing, some 12): 68 % of the issue slots at 38 % of the warps.  A step of 8 tokens 5.9 us, two chains of
+// latencies.
 template <int D, int HEADS>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4AppendParams p, uint32_t items) {
     constexpr int U = D / 8, G = D / kKv4Group;

@@ -8,15 +8,18 @@
 // against -8 times the sums of the query over the groups (in two fp16 parts), takes the offset off.  For v^T p^T (dimensions are the rows) the probabilities, transposed in registers, take the value's
 // scale with them, one B operand per group, and one more MMA per group against a constant of 8 gives what the offset has to
 // take off.  p is relative to the running maximum and to the largest power of two among the values' scales, so that p and p * vs lie in
-// fp16's normal range wherever it matters.
+// fp16's normal range wherever it matters: down to values of 3e-6, where a scale is two of fp16's last places.
+// Probabilities, and their products with the value scales, are rounded to fp16 because that is what the MMA takes; the errors of the results against 64 bits
+// go from 1.66e-3 (their own rounding to bf16) to 1.67e-3.  The MMA lines subnormal operands up as if they were 2^-14, and cuts sums off at some 2^-14 of p vs,
+// an eighth of what that rounding leaves in a value of one step: a value of 0 under one key that has all of the weight comes out as some 2^-17 of the largest.
 //
 // A warp takes 32 tokens at a time by itself: their codes and scales, four contiguous pieces of memory, arrive by cp.async in a ring of
 // three places that is the warp's own, and are read from there in the order in which the fragments want them.  (Bulk copies of 256 bytes to
 // 2 KB, four to a block, came at 1.7 TB/s: the copy engine takes them one by one.)
 //
 // What bounds it is a block's instructions: some 300 for 32 keys of 128 and 8 query rows, of which the MMAs are a fifth of the tensor pipe, at 16 warps
-// an SM and 1.7 instructions a clock.  32 sequences of 8,000 keys, 64 heads over 8: 62 us, 3.6 TB/s of 6.46; 131,000 keys, 20 heads over 5: 35.5 us, 2.7
-// TB/s, the join included; 600 keys 6.3 us, a chain of latencies.
+// an SM and 1.7 instructions a clock.  32 sequences of 8,000 keys, 64 heads over 8: 62 us, 3.6 TB/s of 6.46; 131,000 keys, 20 heads over 5: 33.6 us, 2.8
+// TB/s, the join included; 600 keys 6.5 us, a chain of latencies.
 #pragma once
 #include "kv4.cuh"
 #include "w2_tile.cuh"

@@ -1342,6 +1342,8 @@ static Kv4Plan kv4_plan(int batch, int tokens, int heads, int kv_heads, int keys
     // One place's share of all keys costs some 10 blocks more than a cluster's: results of two items, the join.  It gains where places stay empty, 17 blocks of
     // a hundred that they would have had, since those that are taken go faster: 5 heads of 131,000 keys, 40 CTAs, 108 against 36 us; 32 and 64 sequences of
     // 20,000, 320 CTAs, 122 against 105 and 233 against 188; but 64 of 700, 8 heads, 19 against 43, and 32 of 8,000, 512 CTAs, 61 against 67.
+    // Both sides are of full caches: lengths are on the device, so `keys` is the capacity.  A mostly empty cache pays: 64 sequences of 700 keys, 8 heads, 17 us
+    // with room for up to 8,192 and 41 from 16,384 on; 16, 5 heads, 9 and 16 (from 32,768); one of 600, 6.4 and 10.7 (131,072).
     const long long ctas = items * pl.cluster, waves = (ctas + slots - 1) / slots;
     if (pl.row_tiles == 1 && items * blocks >= 4ll * kKv4Warps * slots && 17 * blocks * (waves * slots - ctas) > 1000ll * slots * pl.cluster) pl.stream = slots, pl.cluster = 1;
     return pl;
