@@ -284,7 +284,7 @@ PyObject* py_kv4_attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
     check_places(c, start, counts);
     const int64_t B = c.batch, T = q0.size(1), H = q0.size(2);
     TORCH_CHECK_VALUE(H % c.kv_heads == 0, H, " query heads over ", c.kv_heads, " key heads");
-    TORCH_CHECK_VALUE(window >= 0 && window <= INT_MAX && scale > 0 && scale <= 1e6, "window ", window, ", scale ", scale);
+    TORCH_CHECK_VALUE(window >= 0 && window <= INT_MAX && (float)scale > 0.f && scale <= 1e6, "window ", window, ", scale ", scale);
     const c10::cuda::CUDAGuard guard(q0.device());
     const Tensor out = at::empty(q0.sizes(), q0.options());
     if (T) {

@@ -217,3 +217,12 @@ def test_strides_of_single_elements_do_not_matter(lib, dtype):
             assert torch.equal(kv4_append(a, x, x, start, q=x, table=table), kv4_append(b, c, c, start, q=c, table=table))
             assert all(torch.equal(s, t) for s, t in zip(a._tensors(), b._tensors())) and torch.equal(kv4_attend(x, a, start), kv4_attend(c, b, start))
     assert lib.ternaspmm_last_status() == 0
+
+
+def test_a_scale_that_fp32_does_not_hold(lib):
+    cache, start = KV4Cache.empty(1, 1, 64, 64), torch.zeros(1, dtype=torch.int64, device="cuda")
+    q = torch.ones((1, 1, 1, 64), device="cuda", dtype=torch.bfloat16)
+    for scale in (1e-50, 0.0, -1.0, 1.1e6, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="scale"):
+            kv4_attend(q, cache, start, scale=scale)
+    assert not kv4_attend(q, cache, start, scale=1e-45).any() and lib.ternaspmm_last_status() == 0
